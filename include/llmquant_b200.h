@@ -281,6 +281,88 @@ int lq_attn_decode_kv_i8_static(const void* q, const int8_t* k_codes, const int8
                                 int Hq, int Hkv, int D, int Tmax, const int64_t* len_dev, int64_t len,
                                 int len_add, float scaling, int splits, int pdl, void* stream);
 
+/* ---------------------------------------------------------------- block-scaled KV cache
+ * A cache for sequences of different lengths, in pages, with ONE fp32 scale per block of tokens
+ * and KV head (the cache above has one per token). Positions are cut into blocks of `block`
+ * tokens. A complete block of one head is [block, head_dim] int8 codes in a page of the pool:
+ * scale = max(amax / 127, 1e-8) over the block, code = clamp(rint(x / scale), -128, 127); a block
+ * that holds a value which is not finite has scale NaN and reads back as NaN. The rows of the
+ * incomplete block and of the one before it are held as they came, in a ring of 2 * block rows per
+ * sequence and head (position p at row p % (2 * block)): a block is quantized once, from the
+ * values that arrived, so the state depends on the tokens and not on how they were cut into
+ * calls, and up to `block` tokens can be taken back by passing a smaller start. head_dim 64 or
+ * 128, block 16, 32, 64 or 128; dtype is the type of the rows that come and go and of the rings.
+ * The table must not name one page twice among the blocks a call completes.
+ * The reference keeps a bf16 cache without pages (llmquant/quantizers/fake.py:39-62): no
+ * counterpart there.
+ *
+ * Every call is about `T_new` rows per sequence on top of `start` cached tokens: sequence b
+ * starts at start_dev[b * start_stride] (start_stride 0 = one value for all) or, with start_dev
+ * NULL, at `start`; the first count_dev[b] of its rows count (cut to [0, T_new]; NULL = all).
+ * Nothing advances by itself: all layers of a step pass the same start. A sequence whose tokens
+ * leave the table, a page id outside the pool and a position outside the angle tables are
+ * skipped (read as NaN) and recorded: lq_block_kv_device_error() returns and clears 2, 1 or 3
+ * (0 = none; it synchronizes with the device). */
+typedef struct lq_block_kv {
+  int8_t* k_pages;        /* [num_pages, kv_heads, block, head_dim], 16-byte aligned */
+  int8_t* v_pages;
+  float* k_scales;        /* [num_pages, kv_heads] */
+  float* v_scales;
+  void* k_ring;           /* [batch, kv_heads, 2 * block, head_dim] of dtype, 16-byte aligned */
+  void* v_ring;
+  const int32_t* table;   /* [batch, max_blocks] page of each block */
+  int64_t num_pages;
+  int max_blocks, batch, kv_heads, head_dim, block, dtype;
+} lq_block_kv;
+int lq_block_kv_device_error(void);
+
+/* New rows [B, H, T_new, D] (element strides of (b, h, t), D contiguous) into the cache. */
+int lq_block_kv_append(const lq_block_kv* cache, const void* k, const void* v, const int64_t* k_strides,
+                       const int64_t* v_strides, int T_new, const int64_t* start_dev, int start_stride,
+                       int64_t start, const int64_t* count_dev, int pdl, void* stream);
+
+/* The cache's values after the call's rows, [B, H, length, D] contiguous: code * scale rounded to
+ * dtype, the incomplete block's rows as they are, zeros behind each sequence. */
+int lq_block_kv_read(const lq_block_kv* cache, void* k_out, void* v_out, int length, const int64_t* start_dev,
+                     int start_stride, int64_t start, const int64_t* count_dev, int T_new, int pdl, void* stream);
+
+/* Norms of queries and keys for each head and the position rotation in one pass, any number of
+ * tokens: y = x * rsqrt(mean(x^2) + eps) * weight over a head's D values (weights [D] of dtype, or
+ * both NULL: no norm), then the first `rot` values turned by the position's angles:
+ * (a, c) -> (a cos - c sin, c cos + a sin) for the pairs (i, i + rot/2), or (2i, 2i + 1) with
+ * `interleaved`. fp32 inside, rounded once. q [B, T, Hq, D] and k [B, T, Hk, D] by element strides
+ * of (b, t, head), the outputs by theirs (in place: the same pointer and strides); Hq or Hk may be
+ * 0. D a multiple of 8 up to 256, rot a multiple of 16 up to D; cos / sin tables fp32
+ * [table_len, rot / 2]; positions int64 by strides of (b, t). A position outside the tables makes
+ * its heads NaN and is recorded as above. transformers' modules round after the norm, after
+ * its weight and twice in the rotation; here nothing is rounded in between. */
+int lq_qk_norm_rope(const void* q, const void* k, const int64_t* q_strides, const int64_t* k_strides, void* q_out,
+                    void* k_out, const int64_t* q_out_strides, const int64_t* k_out_strides, int dtype, int B,
+                    int T_new, int Hq, int Hk, int D, const void* q_weight, const void* k_weight, float eps,
+                    const float* cos_table, const float* sin_table, int64_t table_len, int rot, int interleaved,
+                    const int64_t* positions, int64_t pos_stride_b, int64_t pos_stride_t, int pdl, void* stream);
+
+/* The two above joined, from the fused projection's rows q|k|v [B, T_new, (Hq + 2 Hkv) * D]
+ * (element strides of (b, t)) in one launch: q normed and turned to q_out [B, T_new, Hq, D]
+ * contiguous (zeros for rows behind count), k normed, turned, rounded to dtype and appended, v
+ * appended. The token at row t has position start + t. */
+int lq_block_kv_append_qkv(const lq_block_kv* cache, const void* qkv, int64_t stride_b, int64_t stride_t, void* q_out,
+                           int Hq, int T_new, const void* q_weight, const void* k_weight, float eps,
+                           const float* cos_table, const float* sin_table, int64_t table_len, int rot,
+                           int interleaved, const int64_t* start_dev, int start_stride, int64_t start,
+                           const int64_t* count_dev, int pdl, void* stream);
+
+/* Attention of the newest T_new rows over the cache as it stands after their append: row t of
+ * sequence b sees the positions 0 .. start + t. q [B, T_new, Hq, D] by element strides of
+ * (b, t, head), D contiguous, 16-byte aligned rows; out [B, T_new, Hq, D] contiguous, zeros for
+ * rows behind count. dtype float16 or bfloat16, any Hq / Hkv. `scratch`
+ * (lq_block_attn_scratch_bytes, 16-byte aligned, no initial contents) holds the partial results of
+ * context slices; calls that may overlap need one each. */
+int64_t lq_block_attn_scratch_bytes(const lq_block_kv* cache, int Hq, int T_new);
+int lq_block_attn(const lq_block_kv* cache, const void* q, const int64_t* q_strides, void* out, void* scratch,
+                  int64_t scratch_bytes, int Hq, int T_new, const int64_t* start_dev, int start_stride, int64_t start,
+                  const int64_t* count_dev, float scaling, int pdl, void* stream);
+
 /* ---------------------------------------------------------------- prefill GEMM (tcgen05 / TMEM)
  * out[m, n] = sum_g s_w[n, g] * s_x[m, g] * sum_{k in g} a[m, k] * q[n, k] on the streaming
  * layout, any M (tiles of 128 tokens x 128 features), out [M, N] bf16, bias bf16 or NULL.

@@ -99,10 +99,33 @@ class GemvTp(ctypes.Structure):
     ]
 
 
+class BlockKV(ctypes.Structure):
+    """Mirror of `lq_block_kv` (include/llmquant_b200.h)."""
+
+    _fields_ = [
+        ("k_pages", _P), ("v_pages", _P), ("k_scales", _P), ("v_scales", _P), ("k_ring", _P), ("v_ring", _P),
+        ("table", _P), ("num_pages", _L), ("max_blocks", _I), ("batch", _I), ("kv_heads", _I), ("head_dim", _I),
+        ("block", _I), ("dtype", _I),
+    ]
+
+
 TP_PUSH, TP_SUM = 1, 2
 
 _SIGNATURES["lq_wq_gemv_fused"] = [ctypes.POINTER(GemvArgs), _P]
 _SIGNATURES["lq_glue_device_error"] = []
+_BLOCK = ctypes.POINTER(BlockKV)
+_SPAN = [_P, _I, _L, _P]  # start_dev, start_stride, start, count_dev
+_ROPE = [ctypes.c_float, _P, _P, _L, _I, _I]  # eps, cos, sin, table_len, rot, interleaved
+_SIGNATURES.update({
+    "lq_block_kv_device_error": [],
+    "lq_block_kv_append": [_BLOCK, _P, _P, _P, _P, _I, *_SPAN, _I, _P],
+    "lq_block_kv_read": [_BLOCK, _P, _P, _I, *_SPAN, _I, _I, _P],
+    "lq_qk_norm_rope": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, *_ROPE, _P, _L, _L, _I, _P],
+    "lq_block_kv_append_qkv": [_BLOCK, _P, _L, _L, _P, _I, _I, _P, _P, *_ROPE, *_SPAN, _I, _P],
+    "lq_block_attn_scratch_bytes": [_BLOCK, _I, _I],
+    "lq_block_attn": [_BLOCK, _P, _P, _P, _P, _L, _I, _I, *_SPAN, ctypes.c_float, _I, _P],
+})
+_RESTYPE["lq_block_attn_scratch_bytes"] = ctypes.c_int64
 _SIGNATURES["lq_decode_gemm_device_error"] = []
 _SIGNATURES["lq_decode_gemm_workspace_bytes"] = [_I, _I, _I]
 _SIGNATURES["lq_tile_weight_bytes"] = [_I, _I, _I]

@@ -1,0 +1,245 @@
+"""A paged KV cache in 8 bits with one scale for each block of tokens and KV head.
+
+`BlockKVStore` is one layer's cache and the calls on it: `append` (quantize on write), `append_qkv`
+(norms of q and k, rotation and append from the fused projection's rows, one launch), `attend` (any
+number of new tokens, sequences of different lengths) and `read` (the values back). A block is
+quantized once, when its last token arrives; the rows of the incomplete block and of the one
+before it stay as they came in a ring, so the cache depends on the tokens and not on how they were
+cut into calls, and up to a block of tokens is taken back by passing a smaller `start`. The
+layout is `lq_block_kv` of include/llmquant_b200.h.
+
+`BlockKVCache` puts it behind transformers' `Cache`, as `KernelQuantCache` does with the cache that
+has a scale per token; `make_cache_factory(8, block_tokens=64)` makes it. The reference has
+neither pages nor sequences of different lengths (llmquant/quantizers/fake.py:39-62).
+"""
+
+import ctypes
+import functools
+
+import torch
+from transformers.cache_utils import Cache, CacheLayerMixin
+
+from llmquant_b200 import native
+from llmquant_b200.cuda.ops import check_norm_weights, check_rope_tables
+
+BLOCK_TOKENS = (16, 32, 64, 128)
+HEAD_DIMS = (64, 128)
+
+
+class BlockKVStore:
+    """One layer's block-scaled cache over tensors that the caller owns:
+
+      k_pages, v_pages    int8 [pages, kv_heads, block, head_dim]
+      k_scales, v_scales  float32 [pages, kv_heads]
+      k_ring, v_ring      [batch, kv_heads, 2 * block, head_dim], the type of the rows that come and go
+      table               int32 [batch, max_blocks], the page of each block of a sequence
+
+    Every call names the tokens it is about: `start` cached tokens (an int for all sequences, or
+    int64 [batch] / [1] on the device) and `count` new rows that count (None: all of them, or
+    int64 [batch]). Nothing advances by itself. `start` and `count` tensors are read on the GPU: what
+    is wrong in them (tokens beyond the table, page ids outside the pool) is skipped there and
+    raised by `check_device_errors`."""
+
+    def __init__(self, k_pages, v_pages, k_scales, v_scales, k_ring, v_ring, table):
+        tensors = dict(k_pages=k_pages, v_pages=v_pages, k_scales=k_scales, v_scales=v_scales, k_ring=k_ring,
+                       v_ring=v_ring, table=table)
+        for name, t in tensors.items():
+            if not t.is_cuda:
+                raise RuntimeError(f"{name} must be a CUDA tensor: there is no CPU fallback")
+            if t.device != k_pages.device or not t.is_contiguous():
+                raise RuntimeError(f"{name} must be contiguous on {k_pages.device}")
+        if k_pages.dim() != 4 or k_pages.dtype != torch.int8:
+            raise RuntimeError("k_pages must be int8 [pages, kv_heads, block, head_dim]")
+        pages, heads, block, dim = k_pages.shape
+        if block not in BLOCK_TOKENS:
+            raise RuntimeError(f"a block must be one of {BLOCK_TOKENS} tokens, got {block}")
+        if dim not in HEAD_DIMS:
+            raise RuntimeError(f"head_dim must be one of {HEAD_DIMS}, got {dim}")
+        if k_ring.dtype not in native.DTYPE_ID:
+            raise RuntimeError(f"the rings must be float32, float16 or bfloat16, got {k_ring.dtype}")
+        if table.dim() != 2 or table.dtype != torch.int32:
+            raise RuntimeError("table must be int32 [batch, max_blocks]")
+        batch, blocks = table.shape
+        want = dict(v_pages=(k_pages.shape, torch.int8), k_scales=((pages, heads), torch.float32),
+                    v_scales=((pages, heads), torch.float32), k_ring=((batch, heads, 2 * block, dim), k_ring.dtype),
+                    v_ring=((batch, heads, 2 * block, dim), k_ring.dtype))
+        for name, (shape, dtype) in want.items():
+            if tuple(tensors[name].shape) != tuple(shape) or tensors[name].dtype != dtype:
+                raise RuntimeError(f"{name} must be {dtype} {tuple(shape)}, got {tensors[name].dtype} "
+                                   f"{tuple(tensors[name].shape)}")
+        if min(pages, heads, batch, blocks) == 0:
+            raise RuntimeError("the cache has no pages, heads, sequences or blocks")
+        self.k_pages, self.v_pages, self.k_scales, self.v_scales = k_pages, v_pages, k_scales, v_scales
+        self.k_ring, self.v_ring, self.table = k_ring, v_ring, table
+        self.batch, self.max_blocks, self.heads, self.head_dim, self.block = batch, blocks, heads, dim, block
+        self.capacity = blocks * block
+        self.dtype, self.device = k_ring.dtype, k_ring.device
+        desc = native.BlockKV(k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+                              k_ring.data_ptr(), v_ring.data_ptr(), table.data_ptr(), pages, blocks, batch, heads, dim,
+                              block, native.DTYPE_ID[self.dtype])
+        self._desc, self._ref = desc, ctypes.byref(desc)
+        self._scratch_bytes = {}
+
+    @classmethod
+    def allocate(cls, batch, kv_heads, head_dim, max_tokens, block_tokens=64, dtype=torch.bfloat16, device="cuda"):
+        """An empty cache of `max_tokens` positions for each of `batch` sequences, with pages of its own."""
+        if block_tokens not in BLOCK_TOKENS:
+            raise RuntimeError(f"a block must be one of {BLOCK_TOKENS} tokens, got {block_tokens}")
+        blocks = -(-max_tokens // block_tokens)
+        pages = batch * blocks
+        codes = [torch.zeros(pages, kv_heads, block_tokens, head_dim, dtype=torch.int8, device=device) for _ in range(2)]
+        scales = [torch.zeros(pages, kv_heads, dtype=torch.float32, device=device) for _ in range(2)]
+        rings = [torch.zeros(batch, kv_heads, 2 * block_tokens, head_dim, dtype=dtype, device=device) for _ in range(2)]
+        table = torch.arange(pages, dtype=torch.int32, device=device).reshape(batch, blocks)
+        return cls(*codes, *scales, *rings, table)
+
+    def _span(self, start, count, tokens):
+        """(start_dev, start_stride, start, count_dev) of the C calls."""
+        if isinstance(start, torch.Tensor):
+            if start.dtype != torch.int64 or start.device != self.device or start.dim() != 1 or \
+                    start.shape[0] not in (1, self.batch):
+                raise RuntimeError(f"start must be an int or int64 [{self.batch}] (or [1]) on {self.device}")
+            span = (start.data_ptr(), start.stride(0) if start.shape[0] == self.batch else 0, 0)
+        else:
+            if not 0 <= start <= self.capacity - (tokens if count is None else 0):
+                raise RuntimeError(f"tokens {start} .. {start + tokens} do not fit a cache of {self.capacity}")
+            span = (0, 0, start)
+        if count is None:
+            return (*span, 0)
+        if not isinstance(count, torch.Tensor) or count.dtype != torch.int64 or count.device != self.device or \
+                count.shape != (self.batch,) or not count.is_contiguous():
+            raise RuntimeError(f"count must be None or a contiguous int64 [{self.batch}] on {self.device}")
+        return (*span, count.data_ptr())
+
+    def _call(self, name, *args):
+        if torch.cuda.current_device() == self.device.index:
+            native.call(name, self._ref, *args, native.stream_ptr(self.device))
+        else:
+            with torch.cuda.device(self.device):
+                native.call(name, self._ref, *args, native.stream_ptr(self.device))
+
+    def _rows(self, t, name, shape):
+        if t.dtype != self.dtype or t.device != self.device:
+            raise RuntimeError(f"{name} must be {self.dtype} on {self.device}, got {t.dtype} on {t.device}")
+        if tuple(t.shape) != shape:
+            raise RuntimeError(f"{name} must be {shape}, got {tuple(t.shape)}")
+
+    def append(self, k, v, start, count=None, pdl=False):
+        """Store new rows k, v [batch, kv_heads, tokens, head_dim] (any strides, head_dim contiguous)."""
+        if k.dim() != 4:
+            raise RuntimeError(f"k must be [batch, kv_heads, tokens, head_dim], got {tuple(k.shape)}")
+        tokens = k.shape[2]
+        shape = (self.batch, self.heads, tokens, self.head_dim)
+        self._rows(k, "k", shape)
+        self._rows(v, "v", shape)
+        span = self._span(start, count, tokens)
+        if tokens == 0:
+            return
+        k = k if k.stride(3) == 1 else k.contiguous()
+        v = v if v.stride(3) == 1 else v.contiguous()
+        self._call("lq_block_kv_append", k.data_ptr(), v.data_ptr(), (ctypes.c_int64 * 3)(*k.stride()[:3]),
+                   (ctypes.c_int64 * 3)(*v.stride()[:3]), tokens, *span, int(pdl))
+
+    def append_qkv(self, qkv, cos, sin, start, count=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False,
+                   q_out=None, pdl=False):
+        """From the fused projection's rows qkv [batch, tokens, q heads + 2 kv heads, head_dim]: queries and
+        keys normed (weights given) and turned by their positions' angles, keys and values stored,
+        queries returned as [batch, tokens, q heads, head_dim]. One launch; the same values as
+        `qk_norm_rope` followed by `append`."""
+        if qkv.dim() != 4 or qkv.shape[2] <= 2 * self.heads:
+            raise RuntimeError(f"qkv must be [batch, tokens, q heads + {2 * self.heads}, head_dim], got {tuple(qkv.shape)}")
+        tokens, heads = qkv.shape[1], qkv.shape[2] - 2 * self.heads
+        self._rows(qkv, "qkv", (self.batch, tokens, heads + 2 * self.heads, self.head_dim))
+        rot = check_rope_tables(cos, sin, self.device, self.head_dim)
+        check_norm_weights(q_weight, k_weight, self.dtype, self.device, self.head_dim)
+        if isinstance(start, int) and start + tokens > cos.shape[0]:
+            raise RuntimeError(f"tokens {start} .. {start + tokens} have no angles in tables of {cos.shape[0]} positions")
+        span = self._span(start, count, tokens)
+        if qkv.stride(3) != 1 or qkv.stride(2) != self.head_dim:
+            qkv = qkv.contiguous()
+        shape = (self.batch, tokens, heads, self.head_dim)
+        if q_out is None:
+            q_out = torch.empty(shape, dtype=self.dtype, device=self.device)
+        else:
+            self._rows(q_out, "q_out", shape)
+            if not q_out.is_contiguous():
+                raise RuntimeError("q_out must be contiguous")
+        if tokens == 0:
+            return q_out
+        self._call("lq_block_kv_append_qkv", qkv.data_ptr(), qkv.stride(0), qkv.stride(1), q_out.data_ptr(), heads,
+                   tokens, native.ptr(q_weight), native.ptr(k_weight), eps, cos.data_ptr(), sin.data_ptr(),
+                   cos.shape[0], rot, int(interleaved), *span, int(pdl))
+        return q_out
+
+    def scratch_bytes(self, q_heads, tokens):
+        """Bytes of scratch one `attend` call of this shape takes."""
+        key = (q_heads, tokens)
+        need = self._scratch_bytes.get(key)
+        if need is None:
+            need = native.library().lq_block_attn_scratch_bytes(self._ref, q_heads, tokens)
+            if need < 0:
+                raise RuntimeError(native.last_error())
+            self._scratch_bytes[key] = need
+        return need
+
+    def attend(self, q, start, count=None, scaling=None, out=None, scratch=None, pdl=False):
+        """Attention of the newest rows q [batch, tokens, q heads, head_dim] (head_dim contiguous) over the
+        cache after their `append`: row t sees positions 0 .. start + t. Returns [batch, tokens,
+        q heads, head_dim], zeros for rows behind `count`. float16 and bfloat16 caches. `scratch`
+        (uint8, `scratch_bytes`) comes from torch's allocator unless given; two calls that may
+        overlap must not share one."""
+        if q.dim() != 4:
+            raise RuntimeError(f"q must be [batch, tokens, q heads, head_dim], got {tuple(q.shape)}")
+        tokens, heads = q.shape[1], q.shape[2]
+        shape = (self.batch, tokens, heads, self.head_dim)
+        self._rows(q, "q", shape)
+        if self.dtype == torch.float32:
+            raise RuntimeError("attention over the block-scaled cache is built for float16 and bfloat16 rows")
+        if heads == 0 or heads % self.heads:
+            raise RuntimeError(f"{heads} query heads do not share {self.heads} KV heads evenly")
+        span = self._span(start, count, tokens)
+        if out is None:
+            out = torch.empty(shape, dtype=self.dtype, device=self.device)
+        else:
+            self._rows(out, "out", shape)
+            if not out.is_contiguous():
+                raise RuntimeError("out must be contiguous")
+        if tokens == 0:
+            return out
+        if q.stride(3) != 1:
+            q = q.contiguous()
+        need = self.scratch_bytes(heads, tokens)
+        if scratch is None:
+            scratch = torch.empty(need, dtype=torch.uint8, device=self.device)
+        elif scratch.device != self.device or scratch.dtype != torch.uint8 or scratch.numel() < need or \
+                not scratch.is_contiguous():
+            raise RuntimeError(f"scratch must be {need} contiguous uint8 on {self.device}")
+        scaling = self.head_dim ** -0.5 if scaling is None else scaling
+        self._call("lq_block_attn", q.data_ptr(), (ctypes.c_int64 * 3)(*q.stride()[:3]), out.data_ptr(),
+                   scratch.data_ptr(), need, heads, tokens, *span, scaling, int(pdl))
+        return out
+
+    def read(self, length, start, count=None, tokens=0):
+        """(K, V) [batch, kv_heads, length, head_dim]: the values the cache stands for with start + count
+        tokens in it (count None: start + tokens), zeros behind each sequence."""
+        if length < 0:
+            raise RuntimeError(f"length must not be negative, got {length}")
+        span = self._span(start, count, tokens)
+        if count is not None:
+            tokens = self.capacity  # count alone decides
+        shape = (self.batch, self.heads, length, self.head_dim)
+        k = torch.empty(shape, dtype=self.dtype, device=self.device)
+        v = torch.empty(shape, dtype=self.dtype, device=self.device)
+        if length:
+            self._call("lq_block_kv_read", k.data_ptr(), v.data_ptr(), length, *span, tokens, 0)
+        return k, v
+
+    def check_device_errors(self):
+        """Raise if a call since the last check met a bad `start`, `count`, page id or position (reads a
+        device word, so it synchronizes)."""
+        with torch.cuda.device(self.device):
+            word = native.library().lq_block_kv_device_error()
+        if word:
+            what = {1: "a page id outside the pool", 2: "tokens outside the table",
+                    3: "a position outside the angle tables"}.get(word, f"error word {word}")
+            raise RuntimeError(f"block-scaled KV cache: a kernel met {what} and skipped it")
