@@ -290,8 +290,10 @@ int lq_attn_decode_kv_i8_static(const void* q, const int8_t* k_codes, const int8
  * incomplete block and of the one before it are held as they came, in a ring of 2 * block rows per
  * sequence and head (position p at row p % (2 * block)): a block is quantized once, from the
  * values that arrived, so the state depends on the tokens and not on how they were cut into
- * calls, and up to `block` tokens can be taken back by passing a smaller start. head_dim 64 or
- * 128, block 16, 32, 64 or 128; dtype is the type of the rows that come and go and of the rings.
+ * calls, and tokens can be taken back, by passing a smaller start, as far as the ring's rows
+ * reach: to the beginning of the block before the one that was incomplete when the cache was
+ * longest. head_dim 64 or 128, block 16, 32, 64 or 128; dtype is the type of the rows that come
+ * and go and of the rings.
  * The table must not name one page twice among the blocks a call completes.
  * The reference keeps a bf16 cache without pages (llmquant/quantizers/fake.py:39-62): no
  * counterpart there.

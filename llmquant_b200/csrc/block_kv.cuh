@@ -5,8 +5,8 @@
 // [batch, max_blocks] names. The rows of the incomplete block, and of the block before it, are
 // held as they came in a ring of 2P rows per sequence and head: position p lives at row p % 2P.
 // So a block is quantized once, from the values that arrived, when its last token arrives: the
-// stored state depends on the tokens alone, not on how they were cut into calls, and up to P
-// tokens can be taken back without loss.
+// stored state depends on the tokens alone, not on how they were cut into calls, and tokens can
+// be taken back without loss as far as the ring reaches.
 #pragma once
 
 #include "common.cuh"

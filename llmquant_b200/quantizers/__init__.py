@@ -8,7 +8,7 @@ from llmquant_b200.quantizers.kernel import (
     quantize_weight_canonical,
 )
 
-from llmquant_b200.quantizers.block_kv import BlockKVStore
+from llmquant_b200.quantizers.block_kv import BlockKVCache, BlockKVLayer, BlockKVStore
 from llmquant_b200.quantizers.experts import KernelQuantExperts, quantize_expert_stack
 from llmquant_b200.quantizers.kv_cache import (
     KernelQuantCache,
@@ -28,7 +28,7 @@ def quant_linear_for(mode: str):
 
 
 __all__ = [
-    "AVAILABLE_MODES", "BlockKVStore", "DECODE_MAX_ROWS", "KERNEL_MAX_ROWS", "KernelQuantCache", "KernelQuantExperts",
+    "AVAILABLE_MODES", "BlockKVCache", "BlockKVLayer", "BlockKVStore", "DECODE_MAX_ROWS", "KERNEL_MAX_ROWS", "KernelQuantCache", "KernelQuantExperts",
     "KernelQuantLinear", "quantize_expert_stack",
     "QuantizedKVLayer", "enable_fused_kv_attention", "make_cache_factory",
     "pad_activation", "quant_linear_for", "quantize_weight_canonical",

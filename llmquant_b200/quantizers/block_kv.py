@@ -5,7 +5,7 @@
 number of new tokens, sequences of different lengths) and `read` (the values back). A block is
 quantized once, when its last token arrives; the rows of the incomplete block and of the one
 before it stay as they came in a ring, so the cache depends on the tokens and not on how they were
-cut into calls, and up to a block of tokens is taken back by passing a smaller `start`. The
+cut into calls, and a smaller `start` takes tokens back without loss as far as the ring reaches. The
 layout is `lq_block_kv` of include/llmquant_b200.h.
 
 `BlockKVCache` puts it behind transformers' `Cache`, as `KernelQuantCache` does with the cache that
@@ -243,3 +243,169 @@ class BlockKVStore:
             what = {1: "a page id outside the pool", 2: "tokens outside the table",
                     3: "a position outside the angle tables"}.get(word, f"error word {word}")
             raise RuntimeError(f"block-scaled KV cache: a kernel met {what} and skipped it")
+
+
+class BlockKVLayer(CacheLayerMixin):
+    """One layer of `BlockKVCache`: a `BlockKVStore` that all sequences fill alike and that grows."""
+
+    is_sliding = False
+    is_compileable = False
+    num_bits = 8
+
+    def __init__(self, block_tokens: int = 64, max_cache_len=None, fused_read: bool = False):
+        super().__init__()
+        if block_tokens not in BLOCK_TOKENS:
+            raise ValueError(f"a block must be one of {BLOCK_TOKENS} tokens, got {block_tokens}")
+        self.block_tokens = block_tokens
+        self.max_cache_len = max_cache_len
+        self.fused_read = fused_read
+        self.dequant_calls = self.fused_reads = 0  # how the cache has been read so far
+        self._length = 0
+        self._ring_from = 0  # the first position whose row as it came is still in the ring
+        self.store = None
+
+    @property
+    def length(self):
+        return self._length
+
+    @length.setter
+    def length(self, value):
+        """More tokens were stored (here, or by a decoder that writes through `store`)."""
+        self._length = value
+        self._ring_from = max(self._ring_from, (value // self.block_tokens - 1) * self.block_tokens)
+
+    def lazy_initialization(self, key_states, value_states):
+        if not key_states.is_cuda:
+            raise RuntimeError("the quantized KV cache needs CUDA tensors: there is no CPU fallback")
+        native.library()
+        self.dtype, self.device = key_states.dtype, key_states.device
+        self.batch, self.heads, _, self.head_dim = key_states.shape
+        self._allocate(self.max_cache_len or 256)
+        self.is_initialized = True
+
+    def _allocate(self, tokens):
+        old = self.store
+        self.store = BlockKVStore.allocate(self.batch, self.heads, self.head_dim, tokens, self.block_tokens, self.dtype,
+                                           self.device)
+        if old is not None:  # each sequence's pages are its own and in order
+            for name in ("k_pages", "v_pages", "k_scales", "v_scales"):
+                dst, src = getattr(self.store, name), getattr(old, name)
+                dst.unflatten(0, (self.batch, -1))[:, : old.max_blocks] = src.unflatten(0, (self.batch, -1))
+            self.store.k_ring, self.store.v_ring = old.k_ring, old.v_ring
+            self.store = BlockKVStore(*(getattr(self.store, n) for n in (
+                "k_pages", "v_pages", "k_scales", "v_scales", "k_ring", "v_ring", "table")))
+
+    @property
+    def capacity(self):
+        return 0 if self.store is None else (self.max_cache_len or self.store.capacity)
+
+    def append(self, key_states, value_states):
+        """Store new tokens of every sequence; returns nothing."""
+        if not self.is_initialized:
+            self.lazy_initialization(key_states, value_states)
+        need = self.length + key_states.shape[-2]
+        if need > self.capacity:
+            if self.max_cache_len is not None:
+                raise RuntimeError(f"KV cache of {self.max_cache_len} tokens cannot take {need}")
+            self._allocate(max(need, 2 * self.capacity))
+        self.store.append(key_states, value_states, self.length)
+        self.length = need
+
+    def dequantized(self, length=None):
+        """(K, V) in the model dtype, [B, H, length, D]."""
+        self.dequant_calls += 1
+        return self.store.read(self.length if length is None else length, self.length)
+
+    def update(self, key_states, value_states, *args, **kwargs):
+        self.append(key_states, value_states)
+        if not self.fused_read:
+            return self.dequantized()
+        # stand-ins of the right shape, tagged so that int_kv_attention knows what it was given
+        shape = (self.batch, self.heads, self.length, self.head_dim)
+        k, v = (r[:, :, :1].expand(shape) for r in (self.store.k_ring, self.store.v_ring))
+        k.lq_layer = v.lq_layer = self
+        return k, v
+
+    def attend(self, q, scaling):
+        """Attention of the newest rows q [B, tokens, Hq, D] over the cache, [B, tokens, Hq, D]."""
+        self.fused_reads += 1
+        return self.store.attend(q, self.length - q.shape[1], scaling=scaling)
+
+    def get_mask_sizes(self, query_length: int):
+        return self.get_seq_length() + query_length, 0
+
+    def get_seq_length(self) -> int:
+        return self.length
+
+    def get_max_cache_shape(self) -> int:
+        return self.max_cache_len if self.max_cache_len is not None else -1
+
+    def reset(self):
+        self._length = self._ring_from = 0
+
+    def crop(self, max_length: int):
+        """Forget the tokens behind `max_length`. Within the ring (the incomplete block and the one before
+        it) nothing is lost; further back the rows of the block that becomes the incomplete one are
+        the values its codes stand for."""
+        if max_length < 0:
+            max_length = self.length - abs(max_length)
+        length = min(self.length, max(max_length, 0))
+        first = length - length % self.block_tokens
+        if first < self._ring_from:
+            if first < length:
+                slots = torch.arange(first, length, device=self.device) % (2 * self.block_tokens)
+                for ring, values in zip((self.store.k_ring, self.store.v_ring), self.store.read(length, self.length)):
+                    ring[:, :, slots] = values[:, :, first:]
+            self._ring_from = first
+        self._length = length
+
+    def offload(self):
+        pass
+
+    def prefetch(self):
+        pass
+
+    def reorder_cache(self, beam_idx):
+        if self.length:
+            idx = beam_idx.to(self.device)
+            for name in ("k_pages", "v_pages", "k_scales", "v_scales"):
+                t = getattr(self.store, name)
+                t.copy_(t.unflatten(0, (self.batch, -1)).index_select(0, idx).flatten(0, 1))
+            for t in (self.store.k_ring, self.store.v_ring):
+                t.copy_(t.index_select(0, idx))
+
+
+class BlockKVCache(Cache):
+    """`Cache` whose layers hold 8-bit codes with one scale per block of tokens and KV head."""
+
+    num_bits = 8
+
+    def __init__(self, block_tokens: int = 64, max_cache_len=None, fused_read: bool = False):
+        if block_tokens not in BLOCK_TOKENS:
+            raise ValueError(f"a block must be one of {BLOCK_TOKENS} tokens, got {block_tokens}")
+        super().__init__(layer_class_to_replicate=functools.partial(BlockKVLayer, block_tokens, max_cache_len, fused_read))
+        self.block_tokens = block_tokens
+        self.capacity_limit = max_cache_len
+        self.fused_read = fused_read
+
+    def crop(self, max_length: int):
+        for layer in self.layers:
+            layer.crop(max_length)
+
+
+# Query tokens up to which `int_kv_attention` reads the codes; longer chunks read the cache back once
+# and take transformers' SDPA.
+ATTEND_TOKENS = 64
+
+
+def attend_layer(layer, module, query, attention_mask, dropout, scaling, kwargs):
+    """What `int_kv_attention` does with a `BlockKVLayer`: (output, None), or None where the kernel does
+    not serve the call (a mask, dropout, a window, a long chunk, another dtype)."""
+    heads, tokens = query.shape[1], query.shape[2]
+    if attention_mask is not None or dropout or kwargs.get("sliding_window") is not None or tokens > ATTEND_TOKENS:
+        return None
+    if query.dtype != layer.dtype or layer.dtype == torch.float32 or heads % layer.heads:
+        return None
+    if tokens > 1 and not kwargs.get("is_causal", getattr(module, "is_causal", True)):
+        return None
+    return layer.attend(query.transpose(1, 2), layer.head_dim ** -0.5 if scaling is None else scaling), None

@@ -24,6 +24,7 @@ import torch
 from transformers.cache_utils import Cache, CacheLayerMixin
 
 from llmquant_b200 import native
+from llmquant_b200.quantizers import block_kv
 
 KV_GROUP = 128
 ATTENTION_NAME = "llmquant_b200_int_kv"
@@ -39,6 +40,12 @@ def int_kv_attention(module, query, key, value, attention_mask, dropout=0.0, sca
     if layer is None:
         return sdpa_attention_forward(module, query, key, value, attention_mask, dropout=dropout,
                                       scaling=scaling, **kwargs)
+    if isinstance(layer, block_kv.BlockKVLayer):
+        done = block_kv.attend_layer(layer, module, query, attention_mask, dropout, scaling, kwargs)
+        if done is not None:
+            return done
+        k, v = layer.dequantized()
+        return sdpa_attention_forward(module, query, k, v, attention_mask, dropout=dropout, scaling=scaling, **kwargs)
     batch, heads, q_len, head_dim = query.shape
     groups = heads // layer.heads if heads % layer.heads == 0 else 0
     fused = (q_len == 1 and query.dtype == torch.bfloat16 and head_dim in (64, 128) and groups in (1, 2, 4, 8)
@@ -219,12 +226,20 @@ class KernelQuantCache(Cache):
             layer.crop(max_length)
 
 
-def make_cache_factory(num_bits, max_cache_len=None, model=None):
+def make_cache_factory(num_bits, max_cache_len=None, model=None, block_tokens=None):
     """Zero-arg factory for `generate(past_key_values=...)`, or None to keep the bf16 cache
     (same contract as llmquant/quantizers/fake.py:58-62). With `model` given and switched to
     the dequantize-on-read attention (`enable_fused_kv_attention`), the caches it makes are
-    read as integers by that model's decode steps instead of being dequantized whole."""
+    read as integers by that model's decode steps instead of being dequantized whole.
+    `block_tokens` (16, 32, 64 or 128; num_bits 8) makes the caches block-scaled: one scale per
+    block of tokens and head (`BlockKVCache`) instead of one per token and head."""
     if num_bits is None:
         return None
     fused = model is not None and getattr(getattr(model, "config", None), "_attn_implementation", None) == ATTENTION_NAME
+    if block_tokens is not None:
+        if num_bits != 8:
+            raise ValueError(f"the block-scaled cache holds 8 bits, got num_bits={num_bits}")
+        if block_tokens not in block_kv.BLOCK_TOKENS:
+            raise ValueError(f"a block must be one of {block_kv.BLOCK_TOKENS} tokens, got {block_tokens}")
+        return lambda: block_kv.BlockKVCache(block_tokens, max_cache_len, fused_read=fused)
     return lambda: KernelQuantCache(num_bits, max_cache_len, fused_read=fused)

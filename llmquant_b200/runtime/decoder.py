@@ -16,6 +16,10 @@ tail of the kernel before it. One step is captured into a CUDA graph and replaye
 the write cursor of the KV cache lives in device memory. Prefill runs through the
 transformers modules (eagerly, as in the reference) into the same integer cache.
 
+With `kv_block` the cache is the block-scaled one (`quantizers/block_kv.py`), and the attention block
+is three launches: norms of q and k, RoPE and append of the q|k|v row; attention; the join of its parts.
+That is also the route of models whose attention normalises queries and keys for each head.
+
 The arithmetic (bf16 roundings of RMSNorm, RoPE, SiLU*mul and the residual adds) follows
 transformers' Llama modules, so greedy tokens match the module-by-module path.
 """
@@ -24,6 +28,7 @@ import torch
 
 from llmquant_b200 import native
 from llmquant_b200.core.scheme import QuantizationScheme
+from llmquant_b200.quantizers.block_kv import BlockKVCache
 from llmquant_b200.quantizers.kernel import KernelQuantLinear
 from llmquant_b200.quantizers.kv_cache import KernelQuantCache
 
@@ -70,6 +75,19 @@ def _unwrap(module):
     return getattr(module, "inner", module)
 
 
+def _head_norms(attn, head_dim):
+    """(q weight, k weight, eps) of an attention that normalises queries and keys for each head, None
+    for one without such norms; ValueError for norms of another kind."""
+    q, k = getattr(attn, "q_norm", None), getattr(attn, "k_norm", None)
+    if q is None and k is None:
+        return None
+    weights = [getattr(m, "weight", None) for m in (q, k)]
+    eps = [getattr(m, "variance_epsilon", getattr(m, "eps", None)) for m in (q, k)]
+    if any(w is None or tuple(w.shape) != (head_dim,) for w in weights) or None in eps or eps[0] != eps[1]:
+        raise ValueError("the norms of queries and keys are not RMS norms over head_dim")
+    return (*(w.detach().to(torch.bfloat16).contiguous() for w in weights), eps[0])
+
+
 def supports(model) -> bool:
     """Whether `model` is a Llama-layout decoder fully on kernel-mode linears."""
     try:
@@ -89,6 +107,11 @@ def supports(model) -> bool:
         if not all(isinstance(m, KernelQuantLinear) and m._stream for m in mods):
             return False
     head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
+    try:
+        if len({_head_norms(layer.self_attn, head_dim) is None for layer in layers}) != 1:
+            return False
+    except ValueError:
+        return False
     groups = cfg.num_attention_heads // cfg.num_key_value_heads
     return head_dim in (64, 128) and groups in (1, 2, 4, 8) and cfg.hidden_act == "silu"
 
@@ -98,7 +121,7 @@ class FusedLlamaDecoder:
 
     def __init__(self, model, max_batch: int, max_len: int, kv_bits: int = 8, use_graph: bool = True,
                  pdl: bool = True, tp=None, attn_splits: int = 0, gather_logits: bool = False,
-                 exchange=None, attn_impl: int = 0):
+                 exchange=None, attn_impl: int = 0, kv_block=None):
         if not supports(model):
             raise ValueError("FusedLlamaDecoder needs a Llama-layout model whose attention and MLP "
                              "linears are KernelQuantLinear (head_dim 64/128, silu MLP)")
@@ -120,6 +143,13 @@ class FusedLlamaDecoder:
         self.scaling = self.D ** -0.5
         self.vocab = cfg.vocab_size
         dev, bf16 = self.device, torch.bfloat16
+        # tokens to a block of the block-scaled cache, None for the cache with a scale per token;
+        # the kernel of the latter has no place for norms of q and k
+        normed = _head_norms(model.model.layers[0].self_attn, self.D) is not None
+        self.kv_block = kv_block or (64 if normed else None)
+        if self.kv_block and kv_bits != 8:
+            raise ValueError("the block-scaled KV cache (and with it a model that normalises queries and keys for "
+                             f"each head) holds 8 bits, got kv_bits={kv_bits}")
 
         self.layers = []
         for layer in model.model.layers:
@@ -131,6 +161,7 @@ class FusedLlamaDecoder:
                 "down": _unwrap(mlp.down_proj),
                 "ln1": layer.input_layernorm.weight.detach().to(bf16).contiguous(),
                 "ln2": layer.post_attention_layernorm.weight.detach().to(bf16).contiguous(),
+                "head_norms": _head_norms(attn, self.D) or (None, None, 1e-6),
             })
         self.final_norm = model.model.norm.weight.detach().to(bf16).contiguous()
         self.lm_head = _unwrap(model.lm_head)
@@ -143,6 +174,11 @@ class FusedLlamaDecoder:
             cos, sin = model.model.rotary_emb(probe, positions)
         self.cos = cos[0].to(bf16).contiguous()
         self.sin = sin[0].to(bf16).contiguous()
+        if self.kv_block:  # fp32, one value per pair
+            with torch.no_grad():
+                cos, sin = model.model.rotary_emb(probe.float(), positions)
+            self.cos_half = cos[0, :, : self.D // 2].float().contiguous()
+            self.sin_half = sin[0, :, : self.D // 2].float().contiguous()
 
         B, H = self.B, self.hidden
         inter = self.layers[0]["down"].in_features
@@ -177,7 +213,11 @@ class FusedLlamaDecoder:
         self.attn_impl = attn_impl
         nbytes = native.library().lq_attn_fused_scratch_bytes(B, self.Hq, self.Hkv, self.D, self.splits)
         self.scratch = torch.zeros(-(-nbytes // 4), dtype=torch.float32, device=dev)
-        self.cache = KernelQuantCache(kv_bits, max_cache_len=max_len)
+        if self.kv_block:
+            self.cache = BlockKVCache(self.kv_block, max_cache_len=max_len)
+            self.block_scratch = None  # allocated with the cache's first layer
+        else:
+            self.cache = KernelQuantCache(kv_bits, max_cache_len=max_len)
         # scratch of the tensor-core decode GEMM that batches above 8 rows go through
         self.workspace = None
         from llmquant_b200.quantizers.kernel import DECODE_GEMM_MIN_ROWS
@@ -191,7 +231,8 @@ class FusedLlamaDecoder:
         self.graph = None
         separate_reduce = self.tp is not None and self.exchange is None
         per_linear = 3 if self.decode_gemm else 1  # the decode GEMM is planes, product, finish
-        self.launches_per_step = (len(self.layers) * (4 * per_linear + 1 + (2 if separate_reduce else 0)) + per_linear
+        per_attention = 3 if self.kv_block else 1
+        self.launches_per_step = (len(self.layers) * (4 * per_linear + per_attention + (2 if separate_reduce else 0)) + per_linear
                                   + (2 if self._glue else 0))
         if not self.tp:
             self.allreduce = "none"
@@ -233,7 +274,18 @@ class FusedLlamaDecoder:
                 return
 
     # ------------------------------------------------------------------ one token
-    def _attention(self, cache, pos_ptr, pdl, stream):
+    def _attention(self, spec, cache, pos_ptr, pdl, stream):
+        if self.kv_block:
+            store = cache.store
+            if self.block_scratch is None:
+                self.block_scratch = torch.empty(store.scratch_bytes(self.Hq, 1), dtype=torch.uint8, device=self.device)
+            heads = (self.B, 1, self.Hq, self.D)
+            q_weight, k_weight, eps = spec["head_norms"]
+            store.append_qkv(self.qkv.view(self.B, 1, -1, self.D), self.cos_half, self.sin_half, self.pos,
+                             q_weight=q_weight, k_weight=k_weight, eps=eps, q_out=self.q_rot.view(heads), pdl=pdl)
+            store.attend(self.q_rot.view(heads), self.pos, scaling=self.scaling, out=self.attn.view(heads),
+                         scratch=self.block_scratch, pdl=pdl)
+            return
         native.call("lq_attn_decode_fused", self.qkv.data_ptr(), self.cos.data_ptr(),
                     self.sin.data_ptr(), cache.k_codes.data_ptr(), cache.v_codes.data_ptr(),
                     cache.k_scales.data_ptr(), cache.v_scales.data_ptr(), self.attn.data_ptr(),
@@ -263,7 +315,7 @@ class FusedLlamaDecoder:
                 tp = ex.sum_args(1, h1)
             spec["qkv"].gemv(h0, norm_weight=spec["ln1"], norm_eps=self.eps, pdl=self.pdl, workspace=self.workspace, out=self.qkv, tp=tp)
             yield
-            self._attention(cache, pos_ptr, pdl, stream)
+            self._attention(spec, cache, pos_ptr, pdl, stream)
             yield
             spec["o"].gemv(self.attn, out_dtype=torch.float32, pdl=self.pdl, workspace=self.workspace, tp=ex.push_args(0))
             yield
@@ -302,7 +354,7 @@ class FusedLlamaDecoder:
         pos_ptr = self.pos.data_ptr()
         for spec, cache in zip(self.layers, self.cache.layers):
             spec["qkv"].gemv(cur, norm_weight=spec["ln1"], norm_eps=self.eps, pdl=self.pdl, workspace=self.workspace, out=self.qkv)
-            self._attention(cache, pos_ptr, pdl, stream)
+            self._attention(spec, cache, pos_ptr, pdl, stream)
             self._row_parallel(spec["o"], self.attn, cur, nxt, 0)
             spec["gate_up"].gemv(nxt, norm_weight=spec["ln2"], norm_eps=self.eps, epilogue=1,
                                  pdl=self.pdl, workspace=self.workspace, out=self.act)
@@ -452,6 +504,8 @@ class FusedLlamaDecoder:
         the last check cannot be trusted. Reads device words, so it synchronizes."""
         lib = native.library()
         words = {"gemv": lib.lq_gemv_device_error(), "attention": lib.lq_attn_device_error()}
+        if self.kv_block:
+            words["block cache"] = lib.lq_block_kv_device_error()
         if self.workspace is not None:
             words["decode gemm"] = lib.lq_decode_gemm_device_error()
         if self.tp:

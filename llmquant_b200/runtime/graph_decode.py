@@ -31,14 +31,17 @@ def can_graph(model, cache_factory=None) -> bool:
     # `graphed_generate(model, ids, n)` without saying which cache they meant
     # (llmquant/eval/evaluate.py:186-199). The answer given here is therefore remembered on the
     # model: the next graphed_generate without an explicit `kv_cache_bits` uses that cache.
-    bits = None
+    bits = block = None
     if cache_factory is not None:
         if not fused.supports(model):
             return False  # the integer cache is graphed by the fused decoder only
-        bits = getattr(cache_factory() if callable(cache_factory) else cache_factory, "num_bits", None)
+        cache = cache_factory() if callable(cache_factory) else cache_factory
+        bits = getattr(cache, "num_bits", None)
         if bits is None:
             return False  # some other cache class: not one this library can capture
+        block = getattr(cache, "block_tokens", None)
     model.__dict__["_graph_kv_cache_bits"] = bits
+    model.__dict__["_graph_kv_block_tokens"] = block
     return True
 
 
@@ -102,17 +105,19 @@ class GraphedDecoder:
 
 
 @torch.no_grad()
-def graphed_generate(model, input_ids, max_new_tokens: int, kv_cache_bits=None):
+def graphed_generate(model, input_ids, max_new_tokens: int, kv_cache_bits=None, kv_block_tokens=None):
     """Greedy generation with the decode step replayed; None if it cannot be graphed.
 
-    `kv_cache_bits` selects the integer KV cache (fused decoder); None means the cache the last
-    `can_graph(model, cache_factory)` call was asked about, bf16 KV if there was none."""
-    if kv_cache_bits is None:
-        kv_cache_bits = model.__dict__.get("_graph_kv_cache_bits")  # what can_graph was asked about
+    `kv_cache_bits` selects the integer KV cache (fused decoder), with `kv_block_tokens` the
+    block-scaled one; None means the cache the last `can_graph(model, cache_factory)` call was
+    asked about, bf16 KV if there was none."""
+    if kv_cache_bits is None:  # what can_graph was asked about
+        kv_cache_bits = model.__dict__.get("_graph_kv_cache_bits")
+        kv_block_tokens = kv_block_tokens or model.__dict__.get("_graph_kv_block_tokens")
     if kv_cache_bits:
         from llmquant_b200.quantizers.kv_cache import make_cache_factory
 
-        ok = can_graph(model, make_cache_factory(kv_cache_bits))
+        ok = can_graph(model, make_cache_factory(kv_cache_bits, block_tokens=kv_block_tokens))
     else:
         ok = can_graph(model)
     if not ok:
@@ -120,7 +125,7 @@ def graphed_generate(model, input_ids, max_new_tokens: int, kv_cache_bits=None):
     prompt = input_ids.shape[1]
     if kv_cache_bits:
         dec = fused.FusedLlamaDecoder(model, input_ids.shape[0], prompt + max_new_tokens + 1,
-                                      kv_bits=kv_cache_bits)
+                                      kv_bits=kv_cache_bits, kv_block=kv_block_tokens)
         return dec.generate(input_ids, max_new_tokens)
     dec = GraphedDecoder(model, prompt, max_new_tokens, batch=input_ids.shape[0])
     nxt = dec.prefill(input_ids)

@@ -107,8 +107,9 @@ def pool_store(batch, heads, dim, blocks, block, dtype, seed=0, spare=3):
     return BlockKVStore(*codes, *scales, *rings, table)
 
 
-def check_state(store, model, counts):
-    """Codes, scales and rings against the definition, bit for bit; pages that are not named untouched."""
+def check_state(store, model, counts, ring_from=0):
+    """Codes, scales and rings against the definition, bit for bit. `ring_from`: where the ring begins after
+    tokens were taken back."""
     block = store.block
     for b, total in enumerate(counts):
         for rows, pages, scales, ring in ((model.k[b], store.k_pages, store.k_scales, store.k_ring),
@@ -119,7 +120,7 @@ def check_state(store, model, counts):
             at = store.table[b, :whole].long()
             assert torch.equal(pages[at].cpu().transpose(0, 1).float(), codes)
             assert torch.equal(scales[at].cpu().T, scale)
-            first = max(0, (whole - 1) * block)
+            first = max(ring_from, (whole - 1) * block)
             slots = torch.arange(first, total) % (2 * block)
             assert torch.equal(ring[b].cpu()[:, slots], rows[:, first:])
 
