@@ -118,30 +118,79 @@ __device__ __forceinline__ Place find_place(const lq_block_kv& c, const BlockSpa
   return Place{total, before, c.batch};
 }
 
+// How many CTAs share a line of `total` units: no more than one for each round of its warps, but
+// one for each (sequence, head) where those are more, so that short contexts need no join.
+__device__ __forceinline__ int64_t sharing(int64_t total, int ctas, int64_t heads) {
+  const int64_t rounds = (total + kWarps - 1) / kWarps;
+  return min(min((int64_t)ctas, total), max(rounds, heads));
+}
+
 template <int D, int NT>
-struct Smem {
+struct Cfg {
   static constexpr int kRows = 8 * NT;
-  static constexpr int kQ = D + 4;   // halves to a staged query row: rows 8 bytes apart in the banks
-  static constexpr int kO = D + 4;   // floats to a partial output row
-  static constexpr size_t q_bytes = (size_t)kRows * kQ * 2;
-  static constexpr size_t o_bytes = (size_t)kWarps * kRows * kO * 4;
-  static constexpr size_t ml_bytes = (size_t)kWarps * kRows * 8;
-  static constexpr size_t total = q_bytes + o_bytes + ml_bytes + kRows * 4;
+  static constexpr int kCtas = NT == 1 ? 2 : 1;          // per SM
+  static constexpr int kStages = NT == 1 ? 3 : 6;        // units in a warp's ring
+  static constexpr int kStage = 2 * kUnit * D + 16;      // codes of K, of V, the two scales
+  static constexpr int kQ = D + 4;                       // halves to a staged query row: rows 8 bytes apart in the banks
+  static constexpr int kO = D + 4;                       // floats to a partial output row
+  static constexpr int kOBytes = kRows * kO * 4;         // a warp's partial outputs, in its ring once that is drained
+  static constexpr int kWarpBytes = kStages * kStage > kOBytes ? kStages * kStage : kOBytes;
+  static constexpr size_t kQBytes = (size_t)kRows * kQ * 2;
+  static constexpr size_t kMlBytes = (size_t)kWarps * kRows * 8;
+  static constexpr size_t kTotal = (size_t)kWarps * kWarpBytes + kQBytes + kMlBytes + kRows * 4;
+  static_assert(kWarpBytes % 16 == 0 && kQBytes % 8 == 0, "");
 };
+
+// 16-byte piece `chunk` of row `row` of a staged unit. Pieces are XOR-swizzled so that both readers
+// are free of bank conflicts: the score product's threads (8 rows, pieces 2 q4 + j) and the value
+// product's (rows 2 q4, piece gid).
+template <int D>
+__device__ __forceinline__ uint32_t piece_at(int row, int chunk) {
+  if (D == 128) return (uint32_t)row * 128 + ((chunk ^ (row & 7)) << 4);
+  return (uint32_t)(row >> 1) * 128 + (((((row & 1) << 2) + chunk) ^ ((row & 6))) << 4);
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 lds128m(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ float2 pair_of(uint32_t v);
+template <>
+__device__ __forceinline__ float2 pair_of<__half>(uint32_t v) {
+  return __half22float2(as_h2(v));
+}
+template <>
+__device__ __forceinline__ float2 pair_of<__nv_bfloat16>(uint32_t v) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
 
 // ---------------------------------------------------------------- main kernel
 // grid (CTAs that share the line, row tiles). T is the type of q, out and the ring.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, (Cfg<D, NT>::kCtas))
 block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const T* __restrict__ q, int64_t qsb, int64_t qst,
-                  int64_t qsh, T* __restrict__ out, float* __restrict__ part, float qk_scale, int* error_word) {
-  constexpr int ROWS = 8 * NT, KS = D / 16, MT = D / 16, DPT = D / 8;  // DPT: dims of V a thread owns
-  using SM = Smem<D, NT>;
+                  int64_t qsh, T* __restrict__ out, float* __restrict__ part, float2* __restrict__ part_ml, float qk_scale,
+                  int* error_word) {
+  using C = Cfg<D, NT>;
+  constexpr int ROWS = C::kRows, KS = D / 16, MT = D / 16, DPT = D / 8;  // DPT: dims of V a thread owns
+  constexpr int J = D / 64;                                              // 16-byte pieces of a K row a thread reads
   extern __shared__ __align__(16) uint8_t smem[];
-  __half* q_s = reinterpret_cast<__half*>(smem);
-  float* o_s = reinterpret_cast<float*>(smem + SM::q_bytes);
-  float2* ml_s = reinterpret_cast<float2*>(smem + SM::q_bytes + SM::o_bytes);
-  float* unit_s = reinterpret_cast<float*>(smem + SM::q_bytes + SM::o_bytes + SM::ml_bytes);
+  __half* q_s = reinterpret_cast<__half*>(smem + (size_t)kWarps * C::kWarpBytes);
+  float2* ml_s = reinterpret_cast<float2*>(smem + (size_t)kWarps * C::kWarpBytes + C::kQBytes);
+  float* unit_s = reinterpret_cast<float*>(smem + (size_t)kWarps * C::kWarpBytes + C::kQBytes + C::kMlBytes);
   __shared__ Place place_s;
 
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -150,22 +199,26 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int gid = lane >> 2, q4 = lane & 3;
   const int rt = blockIdx.y, P = c.block;
-  const int ctas = gridDim.x, cta = blockIdx.x;
+  const int cta = blockIdx.x;
+  const int64_t heads = (int64_t)c.batch * c.kv_heads;
   if (warp == 0) {
     const Place p = find_place(c, sp, sh, rt, error_word, [&](int64_t total) {
-      const int64_t n = total < ctas ? total : ctas;
+      const int64_t n = sharing(total, gridDim.x, heads);
       return cta < n ? total * cta / n : total;
     });
     if (lane == 0) place_s = p;
   }
   __syncthreads();
   const int64_t total = place_s.total;
-  const int64_t n_ctas = total < ctas ? total : ctas;
+  const int64_t n_ctas = sharing(total, gridDim.x, heads);
   if (cta >= n_ctas) return;
   int64_t left = total * (cta + 1) / n_ctas - total * cta / n_ctas;
   int64_t off = total * cta / n_ctas - place_s.before;
-  float* my_part = part + (int64_t)rt * (ctas + (int64_t)c.batch * c.kv_heads) * ROWS * (D + 2);
+  const int64_t tile_slot = (int64_t)rt * (gridDim.x + heads) + cta;
+  uint8_t* ring = smem + (size_t)warp * C::kWarpBytes;
+  const uint32_t ring_a = smem_u32(ring);
 
+#pragma unroll 1
   for (int b = place_s.b; left > 0 && b < c.batch; ++b) {
     SeqSpan s;
     bool bad;
@@ -178,14 +231,45 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
     const int t_lo = rt * sh.tile / sh.G, t_hi = min(s.n - 1, (rt * sh.tile + sh.tile - 1) / sh.G);
     const int visible = s.start + t_hi + 1;
     const int code_units = (min(visible, held) + kUnit - 1) / kUnit;
+    const int* table = c.table + (int64_t)b * c.max_blocks;
+#pragma unroll 1
     for (int h = (int)(off / units); h < c.kv_heads && left > 0; ++h) {
       const int ua = (int)(off - (int64_t)h * units);
       const int ub = (int)min((int64_t)units, ua + left);
       off += ub - ua;
       left -= ub - ua;
 
+      // ---- the warp's ring: codes and scales of its units, kStages - 1 of them on their way
+      const int last_code = min(ub, code_units);
+      auto issue = [&](int u, int stage) {
+        if (u < last_code) {
+          const int pos0 = u * kUnit;
+          const int id = table[pos0 / P];
+          const uint32_t dst = ring_a + stage * C::kStage;
+          if (id < 0 || id >= c.num_pages) {
+            if (lane == 0) {
+              atomicExch(error_word, LQ_BLOCK_BAD_PAGE);
+              float* sc = reinterpret_cast<float*>(ring + stage * C::kStage + 2 * kUnit * D);
+              sc[0] = sc[1] = __int_as_float(0x7fffffff);
+            }
+          } else {
+            const int64_t ph = (int64_t)id * c.kv_heads + h;
+            const int64_t at = (ph * P + pos0 % P) * D;
+#pragma unroll
+            for (int i = 0; i < kUnit * D / 512; ++i) {
+              const int idx = i * 32 + lane, row = idx / (D / 16), chunk = idx % (D / 16);
+              cp_async16(dst + piece_at<D>(row, chunk), c.k_pages + at + idx * 16);
+              cp_async16(dst + kUnit * D + piece_at<D>(row, chunk), c.v_pages + at + idx * 16);
+            }
+            if (lane < 2) cp_async4(dst + 2 * kUnit * D + lane * 4, (lane ? c.v_scales : c.k_scales) + ph);
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+#pragma unroll
+      for (int i = 0; i < C::kStages - 1; ++i) issue(ua + warp + i * kWarps, i);
+
       // ---- the tile's query rows as fp16, each lifted by a power of two
-      __syncthreads();  // (the last segment's merge has read the shared memory)
       for (int r = warp; r < ROWS; r += kWarps) {
         const int row = rt * sh.tile + r, t = row / sh.G, g = row % sh.G;
         const bool live = row < sh.rows && t < s.n;
@@ -198,7 +282,7 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
         float unit;
         const float lift = lift_of(warp_max(amax), 10, unit);
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) q_s[r * SM::kQ + lane + 32 * i] = __float2half_rn(x[i] * lift);
+        for (int i = 0; i < D / 32; ++i) q_s[r * C::kQ + lane + 32 * i] = __float2half_rn(x[i] * lift);
         if (lane == 0) unit_s[r] = unit * qk_scale;
       }
       __syncthreads();
@@ -216,8 +300,8 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
           seen[nt][e] = s.start + (rt * sh.tile + r) / sh.G;
         }
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const uint2 v = *reinterpret_cast<const uint2*>(q_s + (nt * 8 + gid) * SM::kQ + (k / 4) * 64 + q4 * 16 + (k % 4) * 4);
+        for (int k = 0; k < KS; ++k) {  // k-step k: the four dims from q4 * 16 J + 4 k on
+          const uint2 v = *reinterpret_cast<const uint2*>(q_s + (nt * 8 + gid) * C::kQ + q4 * 16 * J + k * 4);
           qb[nt][k][0] = v.x;
           qb[nt][k][1] = v.y;
         }
@@ -230,125 +314,21 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
 #pragma unroll
         for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
       }
-      const T* k_ring = reinterpret_cast<const T*>(c.k_ring) + ((int64_t)b * c.kv_heads + h) * 2 * P * D;
-      const T* v_ring = reinterpret_cast<const T*>(c.v_ring) + ((int64_t)b * c.kv_heads + h) * 2 * P * D;
 
-      for (int u = ua + warp; u < ub; u += kWarps) {
-        const bool tail = u >= code_units;
-        const int pos0 = tail ? held + (u - code_units) * kUnit : u * kUnit;
-        uint32_t ka[KS][4];       // K as the A operand: tokens gid, gid + 8
-        uint32_t va[MT][4];       // V^T as the A operand
-        float ks, vs;
-        if (!tail) {
-          const int64_t page = page_of(c, b, pos0 / P);
-          if (page < 0) {
-            if (lane == 0) atomicExch(error_word, LQ_BLOCK_BAD_PAGE);
-            ks = vs = __int_as_float(0x7fffffff);
-          } else {
-            ks = c.k_scales[page * c.kv_heads + h];
-            vs = c.v_scales[page * c.kv_heads + h];
-          }
-          const int64_t at = ((page < 0 ? 0 : page) * c.kv_heads + h) * P + pos0 % P;
-          const int8_t* kp = c.k_pages + (at + gid) * D + q4 * 16;
-          const int8_t* vp = c.v_pages + (at + q4 * 2) * D + gid * DPT;
-          uint32_t kw[2][KS], vw[4][DPT / 4];
-#pragma unroll
-          for (int j = 0; j < D / 64; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint4 v = *reinterpret_cast<const uint4*>(kp + e * 8 * D + j * 64);
-              kw[e][4 * j] = v.x; kw[e][4 * j + 1] = v.y; kw[e][4 * j + 2] = v.z; kw[e][4 * j + 3] = v.w;
-            }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {  // tokens 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9
-            const int8_t* row = vp + ((e & 1) + (e >> 1) * 8) * D;
-            if (DPT == 16) {
-              const uint4 v = *reinterpret_cast<const uint4*>(row);
-              vw[e][0] = v.x; vw[e][1] = v.y; vw[e][DPT / 4 - 2] = v.z; vw[e][DPT / 4 - 1] = v.w;
-            } else {
-              const uint2 v = *reinterpret_cast<const uint2*>(row);
-              vw[e][0] = v.x; vw[e][1] = v.y;
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t w = kw[e][k] ^ 0x80808080u;
-              ka[k][e] = codes_h2(w, 0x4140u);
-              ka[k][e + 2] = codes_h2(w, 0x4342u);
-            }
-          // row gid of tile mt is dim gid * DPT + 2 mt, row gid + 8 the one after it
-#pragma unroll
-          for (int w = 0; w < DPT / 4; ++w)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t x = vw[2 * e][w] ^ 0x80808080u, y = vw[2 * e + 1][w] ^ 0x80808080u;
-              const uint32_t lo = __byte_perm(x, y, 0x5140u), hi = __byte_perm(x, y, 0x7362u);
-              va[2 * w][2 * e] = codes_h2(lo, 0x4140u);
-              va[2 * w][2 * e + 1] = codes_h2(lo, 0x4342u);
-              va[2 * w + 1][2 * e] = codes_h2(hi, 0x4140u);
-              va[2 * w + 1][2 * e + 1] = codes_h2(hi, 0x4342u);
-            }
-        } else {
-          // rows of the incomplete block: lifted by a power of two of their own and taken as fp16
-          // (a bf16 value has 8 significant bits; the smallest are lost 2^-24 below the largest)
-          float kx[2][DPT * 2], vx[4][DPT], kmax = 0.f, vmax = 0.f;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int pos = pos0 + gid + e * 8;
-            const T* row = k_ring + (int64_t)(pos % (2 * P)) * D;
-#pragma unroll
-            for (int i = 0; i < DPT * 2; ++i) {
-              kx[e][i] = pos < L ? Conv<T>::to_f32(row[(i / 16) * 64 + q4 * 16 + i % 16]) : 0.f;
-              kmax = fmaxf(kmax, finite_abs(kx[e][i]));
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int pos = pos0 + q4 * 2 + (e & 1) + (e >> 1) * 8;
-            const T* row = v_ring + (int64_t)(pos % (2 * P)) * D + gid * DPT;
-#pragma unroll
-            for (int i = 0; i < DPT; ++i) {
-              vx[e][i] = pos < L ? Conv<T>::to_f32(row[i]) : 0.f;
-              vmax = fmaxf(vmax, finite_abs(vx[e][i]));
-            }
-          }
-          const float klift = lift_of(warp_max(kmax), 10, ks), vlift = lift_of(warp_max(vmax), 7, vs);
-#pragma unroll
-          for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float* x = &kx[e][k * 4];
-              ka[k][e] = as_u32(__floats2half2_rn(x[0] * klift, x[1] * klift));
-              ka[k][e + 2] = as_u32(__floats2half2_rn(x[2] * klift, x[3] * klift));
-            }
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              va[i][2 * e] = as_u32(__floats2half2_rn(vx[2 * e][2 * i] * vlift, vx[2 * e + 1][2 * i] * vlift));
-              va[i][2 * e + 1] = as_u32(__floats2half2_rn(vx[2 * e][2 * i + 1] * vlift, vx[2 * e + 1][2 * i + 1] * vlift));
-            }
-        }
-
-        // ---- scores, weights
+      // scores of 16 tokens from pos0 on (acc: raw products) to the weights as B operands
+      uint32_t wb[NT][2];
+      auto weigh = [&](float (&acc)[NT][4], int pos0, float ks, float vs) {
         const float lv = __log2f(vs), inv_vs = 1.f / vs;
         const bool masked = pos0 + kUnit - 1 > s.start + t_lo;
-        float x[NT][4];
         bool rises = false;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int k = 0; k < KS; ++k) mma16(acc, ka[k][0], ka[k][1], ka[k][2], ka[k][3], qb[nt][k][0], qb[nt][k][1]);
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            x[nt][i] = fmaf(acc[i], qu[nt][i & 1] * ks, lv);
-            if (masked && pos0 + gid + (i >> 1) * 8 > seen[nt][i & 1]) x[nt][i] = -INFINITY;
-            rises = rises || x[nt][i] > m[nt][i & 1] + 8.f;
+            acc[nt][i] = fmaf(acc[nt][i], qu[nt][i & 1] * ks, lv);
+            if (masked && pos0 + gid + (i >> 1) * 8 > seen[nt][i & 1]) acc[nt][i] = -INFINITY;
+            rises = rises || acc[nt][i] > m[nt][i & 1] + 8.f;
           }
-        }
         // M follows the maximum only when a weight would pass 2^8: any M serves, and fp16 keeps 11
         // bits of a weight up to 2^15
         if (__any_sync(0xffffffffu, rises)) {
@@ -356,7 +336,7 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float mx = fmaxf(x[nt][e], x[nt][e + 2]);
+              float mx = fmaxf(acc[nt][e], acc[nt][e + 2]);
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -377,7 +357,7 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float base = m[nt][i & 1] == -INFINITY ? 0.f : m[nt][i & 1];
-            w[i] = exp2f(x[nt][i] - base);
+            w[i] = exp2f(acc[nt][i] - base);
           }
           // the sum takes the weights as they are multiplied, rounded to fp16: their rounding then
           // cancels where few weights dominate. (Below 2^-14, where fp16 loses bits, it takes them
@@ -389,13 +369,155 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
           const float sum1 = (w[1] < least ? w[1] : f0.y) + (w[3] < least ? w[3] : f1.y);
           l[nt][0] += sum0 == 0.f ? 0.f : sum0 * inv_vs;  // (a masked token's scale may be NaN)
           l[nt][1] += sum1 == 0.f ? 0.f : sum1 * inv_vs;
-          const uint32_t b0 = transpose8x8(as_u32(w0)), b1 = transpose8x8(as_u32(w1));
+          wb[nt][0] = transpose8x8(as_u32(w0));
+          wb[nt][1] = transpose8x8(as_u32(w1));
+        }
+      };
+
+      // ---- complete blocks
+      int stage = 0;
+#pragma unroll 1
+      for (int u = ua + warp; u < last_code; u += kWarps) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 2) : "memory");
+        __syncwarp();  // the unit is there for every lane, and every lane is done with the one before
+        const int behind = stage == 0 ? C::kStages - 1 : stage - 1;
+        issue(u + (C::kStages - 1) * kWarps, behind);
+        const uint32_t k_a = ring_a + stage * C::kStage, v_a = k_a + kUnit * D;
+        const uint2 sc = lds64(v_a + kUnit * D);
+        stage = stage + 1 == C::kStages ? 0 : stage + 1;
+        float acc[NT][4];
 #pragma unroll
-          for (int i = 0; i < MT; ++i) mma16(o[nt][i], va[i][0], va[i][1], va[i][2], va[i][3], b0, b1);
+        for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const uint4 x = lds128m(k_a + piece_at<D>(gid, q4 * J + j)), y = lds128m(k_a + piece_at<D>(gid + 8, q4 * J + j));
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t xw = xs[k] ^ 0x80808080u, yw = ys[k] ^ 0x80808080u;
+            const uint32_t a0 = codes_h2(xw, 0x4140u), a1 = codes_h2(yw, 0x4140u);
+            const uint32_t a2 = codes_h2(xw, 0x4342u), a3 = codes_h2(yw, 0x4342u);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16(acc[nt], a0, a1, a2, a3, qb[nt][4 * j + k][0], qb[nt][4 * j + k][1]);
+          }
+        }
+        weigh(acc, u * kUnit, __uint_as_float(sc.x), __uint_as_float(sc.y));
+        // row gid of value tile i is dim gid * DPT + 2 i, row gid + 8 the one after it
+        uint32_t vw[4][DPT / 4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // tokens 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9
+          const int row = q4 * 2 + (e & 1) + (e >> 1) * 8;
+          if (D == 128) {
+            const uint4 v = lds128m(v_a + piece_at<D>(row, gid));
+            vw[e][0] = v.x; vw[e][1] = v.y; vw[e][DPT / 4 - 2] = v.z; vw[e][DPT / 4 - 1] = v.w;
+          } else {
+            const uint2 v = lds64(v_a + piece_at<D>(row, gid >> 1) + (gid & 1) * 8);
+            vw[e][0] = v.x; vw[e][1] = v.y;
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < DPT / 4; ++w) {
+          uint32_t a[2][4];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t x = vw[2 * e][w] ^ 0x80808080u, y = vw[2 * e + 1][w] ^ 0x80808080u;
+            const uint32_t lo = __byte_perm(x, y, 0x5140u), hi = __byte_perm(x, y, 0x7362u);
+            a[0][2 * e] = codes_h2(lo, 0x4140u);
+            a[0][2 * e + 1] = codes_h2(lo, 0x4342u);
+            a[1][2 * e] = codes_h2(hi, 0x4140u);
+            a[1][2 * e + 1] = codes_h2(hi, 0x4342u);
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16(o[nt][2 * w + i], a[i][0], a[i][1], a[i][2], a[i][3], wb[nt][0], wb[nt][1]);
         }
       }
 
-      // ---- merge the warps
+      // ---- rows of the incomplete block: lifted by a power of two of their own and taken as fp16 (a
+      // bf16 value has 8 significant bits; what is lost lies 2^-24 below the largest)
+      const int first_tail = max(ua, code_units);
+      const int skew = (first_tail - ua - warp) & (kWarps - 1);  // units go round the warps without a break
+#pragma unroll 1
+      for (int u = first_tail + ((kWarps - skew) & (kWarps - 1)); u < ub; u += kWarps) {
+        const int pos0 = held + (u - code_units) * kUnit;
+        const int64_t bh = ((int64_t)b * c.kv_heads + h) * 2 * P;
+        float acc[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+        uint4 kx[2][2 * J];
+        float kmax = 0.f, vmax = 0.f;
+        auto largest = [](const uint4& v, float& top) {
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 p = pair_of<T>(w[i]);
+            top = fmaxf(top, fmaxf(finite_abs(p.x), finite_abs(p.y)));
+          }
+        };
+        auto row_of = [&](const void* rows, int pos) {
+          return reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(rows) + (bh + pos % (2 * P)) * D);
+        };
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int pos = pos0 + gid + e * 8;
+          const uint4* row = row_of(c.k_ring, pos) + q4 * 2 * J;
+#pragma unroll
+          for (int i = 0; i < 2 * J; ++i) {
+            kx[e][i] = pos < L ? row[i] : make_uint4(0u, 0u, 0u, 0u);
+            largest(kx[e][i], kmax);
+          }
+        }
+        // (the values are read twice, the second time from L1: once for their maximum, once to multiply)
+        auto value_piece = [&](int e, int i) {
+          const int pos = pos0 + q4 * 2 + (e & 1) + (e >> 1) * 8;
+          return pos < L ? row_of(c.v_ring, pos)[gid * (DPT / 8) + i] : make_uint4(0u, 0u, 0u, 0u);
+        };
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int i = 0; i < DPT / 8; ++i) largest(value_piece(e, i), vmax);
+        float ks, vs;
+        const float klift = lift_of(warp_max(kmax), 10, ks), vlift = lift_of(warp_max(vmax), 7, vs);
+        auto lifted = [](uint32_t v, float lift) {
+          const float2 p = pair_of<T>(v);
+          return as_u32(__floats2half2_rn(p.x * lift, p.y * lift));
+        };
+#pragma unroll
+        for (int i = 0; i < 2 * J; ++i) {  // 8 dims: k-steps 2 i, 2 i + 1
+          const uint32_t xs[4] = {kx[0][i].x, kx[0][i].y, kx[0][i].z, kx[0][i].w};
+          const uint32_t ys[4] = {kx[1][i].x, kx[1][i].y, kx[1][i].z, kx[1][i].w};
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t a0 = lifted(xs[2 * k], klift), a1 = lifted(ys[2 * k], klift);
+            const uint32_t a2 = lifted(xs[2 * k + 1], klift), a3 = lifted(ys[2 * k + 1], klift);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16(acc[nt], a0, a1, a2, a3, qb[nt][2 * i + k][0], qb[nt][2 * i + k][1]);
+          }
+        }
+        weigh(acc, pos0, ks, vs);
+#pragma unroll
+        for (int i = 0; i < DPT / 8; ++i) {
+          uint32_t y[4][4];  // [token][pair of dims], lifted
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint4 v = value_piece(e, i);
+            y[e][0] = lifted(v.x, vlift); y[e][1] = lifted(v.y, vlift);
+            y[e][2] = lifted(v.z, vlift); y[e][3] = lifted(v.w, vlift);
+          }
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {  // value tile 4 i + d: dims 2 d, 2 d + 1 of the eight
+            const uint32_t a0 = __byte_perm(y[0][d], y[1][d], 0x5410u), a1 = __byte_perm(y[0][d], y[1][d], 0x7632u);
+            const uint32_t a2 = __byte_perm(y[2][d], y[3][d], 0x5410u), a3 = __byte_perm(y[2][d], y[3][d], 0x7632u);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16(o[nt][4 * i + d], a0, a1, a2, a3, wb[nt][0], wb[nt][1]);
+          }
+        }
+      }
+
+      // ---- merge the warps, each one's outputs in its drained ring
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -406,107 +528,131 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
           sum += __shfl_xor_sync(0xffffffffu, sum, 16);
           const int r = nt * 8 + q4 * 2 + e;
           if (gid == 0) ml_s[warp * ROWS + r] = make_float2(m[nt][e], sum);
-          float* dst = o_s + (warp * ROWS + r) * SM::kO + gid * DPT;
+          float* dst = reinterpret_cast<float*>(ring) + r * C::kO + gid * DPT;
 #pragma unroll
           for (int i = 0; i < MT; ++i) *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[nt][i][e], o[nt][i][e + 2]);
         }
       __syncthreads();
       const bool whole = ua == 0 && ub == units;
-      float* dst_part = my_part + (cta + (int64_t)b * c.kv_heads + h) * ROWS * (D + 2);
-      for (int i = threadIdx.x; i < ROWS * D; i += kThreads) {
-        const int r = i / D, d = i % D;
+      const int64_t slot = tile_slot + (int64_t)b * c.kv_heads + h;
+      for (int i = threadIdx.x; i < ROWS * D / 4; i += kThreads) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        const int row = rt * sh.tile + r, t = row / sh.G, g = row % sh.G;
+        if (row >= sh.rows) break;  // (rows rise with i)
         float top = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml_s[w * ROWS + r].x);
-        float sum = 0.f, acc = 0.f;
+        float sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
           const float2 ml = ml_s[w * ROWS + r];
           // (a warp without units has -inf; one whose scores are NaN has NaN sums and must count)
           const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2f(ml.x - top);
+          const float4 v = *reinterpret_cast<const float4*>(smem + (size_t)w * C::kWarpBytes + ((size_t)r * C::kO + d) * 4);
           sum = fmaf(ml.y, f, sum);
-          acc = fmaf(o_s[(w * ROWS + r) * SM::kO + d], f, acc);
+          acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y);
+          acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
         }
         if (whole) {
-          const int row = rt * sh.tile + r, t = row / sh.G, g = row % sh.G;
-          if (row < sh.rows)
-            out[(((int64_t)b * sp.tokens + t) * sh.Hq + h * sh.G + g) * D + d] =
-                Conv<T>::from_f32(t < s.n ? acc / sum : 0.f);
+          T* dst = out + (((int64_t)b * sp.tokens + t) * sh.Hq + h * sh.G + g) * D + d;
+          const float inv = t < s.n ? 1.f / sum : 0.f;
+          const bool live = t < s.n;
+          dst[0] = Conv<T>::from_f32(live ? acc.x * inv : 0.f);
+          dst[1] = Conv<T>::from_f32(live ? acc.y * inv : 0.f);
+          dst[2] = Conv<T>::from_f32(live ? acc.z * inv : 0.f);
+          dst[3] = Conv<T>::from_f32(live ? acc.w * inv : 0.f);
         } else {
-          dst_part[r * (D + 2) + d] = acc;
-          if (d == 0) {
-            dst_part[r * (D + 2) + D] = top;
-            dst_part[r * (D + 2) + D + 1] = sum;
-          }
+          *reinterpret_cast<float4*>(part + (slot * ROWS + r) * D + d) = acc;
+          if (d == 0) part_ml[slot * ROWS + r] = make_float2(top, sum);
         }
       }
+      __syncthreads();  // the shared memory is free for the next (sequence, head)
     }
     off -= (int64_t)units * c.kv_heads;  // zero where the run goes on into the next sequence
   }
 }
 
 // ---------------------------------------------------------------- join the parts
-// grid (KV heads, batch, row tiles), D threads: a (sequence, head) that several CTAs shared is the
-// weighted sum of their parts; one that none took (no rows that count) becomes zeros.
-template <typename T>
-__global__ void block_attn_join_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, int ctas, T* __restrict__ out,
-                                       const float* __restrict__ part, int* error_word) {
-  __shared__ Place place_s;
+// grid (KV heads x rows of a tile, batch, row tiles), four warps: an output row that several CTAs
+// shared is the weighted sum of their parts; one that none took (it does not count) becomes
+// zeros. A warp takes every fourth part, a lane D / 32 of its values.
+constexpr int kJoinWarps = 4;
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinWarps * 32)
+block_attn_join_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, int ctas, T* __restrict__ out,
+                       const float* __restrict__ part, const float2* __restrict__ part_ml) {
+  constexpr int V = D / 32;
+  __shared__ float acc_s[kJoinWarps][D];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int h = blockIdx.x, b = blockIdx.y, rt = blockIdx.z, D = c.head_dim, d = threadIdx.x;
+  const int h = blockIdx.x % c.kv_heads, r = blockIdx.x / c.kv_heads, b = blockIdx.y, rt = blockIdx.z;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = rt * sh.tile + r, t = row / sh.G, g = row % sh.G;
+  if (row >= sh.rows) return;
   // (start and count are older than the kernel ahead, which has waited for their writer)
   SeqSpan s;
   bool bad;
   const int units = units_of(c, sp, sh, b, rt, s, bad);
-  int64_t u0 = 0;
+  const int64_t heads = (int64_t)c.batch * c.kv_heads;
   int c0 = 0, c1 = -1;
-  int64_t total = 0, n = 0;
   if (units > 0) {
-    if (threadIdx.x < 32) {
-      // units before sequence b: ask for the unit that b's first one is
-      int64_t before = 0, all = 0;
-      for (int i = threadIdx.x; i < c.batch; i += 32) {
-        SeqSpan si;
-        bool bi;
-        const int64_t v = (int64_t)units_of(c, sp, sh, i, rt, si, bi) * c.kv_heads;
-        all += v;
-        if (i < b) before += v;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        before += __shfl_xor_sync(0xffffffffu, before, o);
-        all += __shfl_xor_sync(0xffffffffu, all, o);
-      }
-      if (threadIdx.x == 0) place_s = Place{all, before, b};
+    int64_t before = 0, total = 0;
+    for (int i = lane; i < c.batch; i += 32) {
+      SeqSpan si;
+      bool bi;
+      const int64_t v = (int64_t)units_of(c, sp, sh, i, rt, si, bi) * c.kv_heads;
+      total += v;
+      if (i < b) before += v;
     }
-    __syncthreads();
-    total = place_s.total;
-    n = total < ctas ? total : ctas;
-    u0 = place_s.before + (int64_t)h * units;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    const int64_t n = sharing(total, ctas, heads);
+    const int64_t u0 = before + (int64_t)h * units;
     c0 = (int)(((u0 + 1) * n - 1) / total);
     c1 = (int)(((u0 + units) * n - 1) / total);
   }
+  T* dst = out + (((int64_t)b * sp.tokens + t) * sh.Hq + h * sh.G + g) * D;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (units > 0 && c0 == c1) return;  // one CTA had all of it and wrote the output
-  const float* mine = part + ((int64_t)rt * (ctas + (int64_t)c.batch * c.kv_heads) + (int64_t)b * c.kv_heads + h) * sh.tile * (D + 2);
-  const int64_t stride = (int64_t)sh.tile * (D + 2);
-  for (int r = 0; r < sh.tile; ++r) {
-    const int row = rt * sh.tile + r, t = row / sh.G, g = row % sh.G;
-    if (row >= sh.rows) break;
-    float v = 0.f;
-    if (units > 0 && t < s.n) {
-      float top = -INFINITY;
-      for (int k = c0; k <= c1; ++k) top = fmaxf(top, mine[k * stride + r * (D + 2) + D]);
-      float sum = 0.f, acc = 0.f;
-      for (int k = c0; k <= c1; ++k) {
-        const float mk = mine[k * stride + r * (D + 2) + D], lk = mine[k * stride + r * (D + 2) + D + 1];
-        const float f = mk == -INFINITY ? (lk == 0.f ? 0.f : 1.f) : exp2f(mk - top);
-        sum = fmaf(lk, f, sum);
-        acc = fmaf(mine[k * stride + r * (D + 2) + d], f, acc);
-      }
-      v = acc / sum;
+  if (units == 0 || t >= s.n) {
+    for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) dst[d] = Conv<T>::from_f32(0.f);
+    return;
+  }
+  const int64_t slot0 = (int64_t)rt * (ctas + heads) + (int64_t)b * c.kv_heads + h + c0;
+  const int parts = c1 - c0 + 1;
+  const float2* ml = part_ml + slot0 * sh.tile + r;
+  const float* mine = part + (slot0 * sh.tile + r) * D + lane * V;
+  float top = -INFINITY;
+  for (int k = lane; k < parts; k += 32) top = fmaxf(top, ml[(int64_t)k * sh.tile].x);
+  top = warp_max(top);
+  float sum = 0.f, acc[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = 0.f;
+#pragma unroll 4
+  for (int k = warp; k < parts; k += kJoinWarps) {
+    const float2 w = ml[(int64_t)k * sh.tile];
+    const float f = w.x == -INFINITY ? (w.y == 0.f ? 0.f : 1.f) : exp2f(w.x - top);
+    const float* v = mine + (int64_t)k * sh.tile * D;
+    sum = fmaf(w.y, f, sum);
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = fmaf(v[i], f, acc[i]);
+  }
+  __shared__ float sum_s[kJoinWarps];
+  if (lane == 0) sum_s[warp] = sum;
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc_s[warp][lane * V + i] = acc[i];
+  __syncthreads();
+  for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) {
+    float v = 0.f, all = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+      v += acc_s[w][d];
+      all += sum_s[w];
     }
-    out[(((int64_t)b * sp.tokens + t) * sh.Hq + h * sh.G + g) * D + d] = Conv<T>::from_f32(v);
+    dst[d] = Conv<T>::from_f32(v / all);
   }
 }
 
@@ -524,14 +670,15 @@ Plan plan_of(const lq_block_kv& c, int Hq, int T_new) {
   p.nt = p.sh.rows <= 8 ? 1 : 2;
   p.sh.tile = 8 * p.nt;
   p.tiles = (p.sh.rows + p.sh.tile - 1) / p.sh.tile;
-  p.ctas = 2 * sm_count() / p.tiles;
+  p.ctas = (p.nt == 1 ? 2 : 1) * sm_count() / p.tiles;
   if (p.ctas < 1) p.ctas = 1;
   return p;
 }
 
-int64_t scratch_bytes(const lq_block_kv& c, const Plan& p) {
-  return (int64_t)p.tiles * (p.ctas + (int64_t)c.batch * c.kv_heads) * p.sh.tile * (c.head_dim + 2) * 4;
+int64_t slots_of(const lq_block_kv& c, const Plan& p) {
+  return (int64_t)p.tiles * (p.ctas + (int64_t)c.batch * c.kv_heads) * p.sh.tile;
 }
+int64_t scratch_bytes(const lq_block_kv& c, const Plan& p) { return slots_of(c, p) * (c.head_dim + 2) * 4; }
 
 int check_attn(const lq_block_kv* c, int Hq, int T_new, const char* what) {
   if (const int rc = check_block_kv(c, what)) return rc;
@@ -567,14 +714,17 @@ template <typename T, int D, int NT>
 int run(const lq_block_kv& c, const BlockSpan& sp, const Plan& p, const void* q, const int64_t* qs, void* out, void* scratch,
         float scaling, int pdl, cudaStream_t stream, int* error_word, const char* what) {
   auto kern = block_attn_kernel<T, D, NT>;
-  constexpr size_t smem = Smem<D, NT>::total;
+  constexpr size_t smem = Cfg<D, NT>::kTotal;
   if (const int rc = ensure_smem_limit(reinterpret_cast<const void*>(kern), (int)smem, what)) return rc;
   const float qk_scale = scaling * 1.4426950408889634f;
+  float* part = (float*)scratch;
+  float2* part_ml = (float2*)(part + slots_of(c, p) * D);
   if (const int rc = launch(kern, dim3((unsigned)p.ctas, (unsigned)p.tiles), kThreads, smem, stream, pdl, what, c, sp, p.sh,
-                            (const T*)q, qs[0], qs[1], qs[2], (T*)out, (float*)scratch, qk_scale, error_word))
+                            (const T*)q, qs[0], qs[1], qs[2], (T*)out, part, part_ml, qk_scale, error_word))
     return rc;
-  return launch(block_attn_join_kernel<T>, dim3((unsigned)c.kv_heads, (unsigned)c.batch, (unsigned)p.tiles), D, 0, stream, 1, what,
-                c, sp, p.sh, p.ctas, (T*)out, (const float*)scratch, error_word);
+  const unsigned rows = (unsigned)(p.sh.rows < p.sh.tile ? p.sh.rows : p.sh.tile);
+  return launch(block_attn_join_kernel<T, D>, dim3((unsigned)c.kv_heads * rows, (unsigned)c.batch, (unsigned)p.tiles),
+                kJoinWarps * 32, 0, stream, 1, what, c, sp, p.sh, p.ctas, (T*)out, (const float*)part, (const float2*)part_ml);
 }
 
 template <typename T>

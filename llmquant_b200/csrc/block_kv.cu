@@ -3,48 +3,68 @@
 // step, which does both from the fused q|k|v row in one launch. Layout: block_kv.cuh.
 #include "block_kv.cuh"
 
+#include <cstring>
+
 namespace lq {
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxVec = 8;  // 8-value pieces a thread holds of one block: 128 * 128 / 8 / 256
 
+// 8 consecutive values as they lie in memory, moved as 16-byte words
 template <typename T>
-struct alignas(16) Pack8 {
-  T v[8];
+struct Pack8 {
+  uint4 w[sizeof(T) / 2];
 };
 
-// 8 consecutive values; `vec` = every row of the tensor starts on a 16-byte boundary
+// `vec` = every row of the tensor starts on a 16-byte boundary
 template <typename T>
 __device__ __forceinline__ Pack8<T> load8(const T* p, bool vec) {
   Pack8<T> r;
   if (vec) {
-    r = *reinterpret_cast<const Pack8<T>*>(p);
-  } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.v[i] = p[i];
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = reinterpret_cast<const uint4*>(p)[i];
+  } else {
+    T v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = p[i];
+    memcpy(&r, v, sizeof(r));
   }
   return r;
 }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const Pack8<T>& r, bool vec) {
   if (vec) {
-    *reinterpret_cast<Pack8<T>*>(p) = r;
-  } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = r.v[i];
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r.w[i];
+  } else {
+    T v[8];
+    memcpy(v, &r, sizeof(r));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = v[i];
   }
 }
 template <typename T>
-__device__ __forceinline__ void unpack8(const Pack8<T>& r, float (&x)[8]) {
+__device__ __forceinline__ Pack8<T> zeros8() {
+  Pack8<T> r;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = Conv<T>::to_f32(r.v[i]);
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = make_uint4(0u, 0u, 0u, 0u);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(const Pack8<T>& r, float (&x)[8]) {
+  T v[8];
+  memcpy(v, &r, sizeof(r));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = Conv<T>::to_f32(v[i]);
 }
 template <typename T>
 __device__ __forceinline__ Pack8<T> pack8(const float (&x)[8]) {
-  Pack8<T> r;
+  T v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r.v[i] = Conv<T>::from_f32(x[i]);
+  for (int i = 0; i < 8; ++i) v[i] = Conv<T>::from_f32(x[i]);
+  Pack8<T> r;
+  memcpy(&r, v, sizeof(r));
   return r;
 }
 
@@ -173,8 +193,7 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const NormRopeAr
                                 : p.k + b * p.ks[0] + t * p.ks[1] + (h - p.Hq) * p.ks[2];
         in[u] = load8(src + d0, p.vec);
       } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) in[u].v[i] = Conv<T>::from_f32(0.f);
+        in[u] = zeros8<T>();
       }
     }
 #pragma unroll
@@ -289,9 +308,7 @@ block_append_kernel(const lq_block_kv c, const BlockSpan sp, const AppendArgs<T>
 
   // one 8-value piece of a new row; every lane of the warp calls it
   auto fetch = [&](int pos, bool fresh) {
-    Pack8<T> r;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r.v[i] = Conv<T>::from_f32(0.f);
+    Pack8<T> r = zeros8<T>();
     if (fresh) r = load8(src + (int64_t)(pos - s.start) * step + li * 8, p.vec);
     if (turned) {
       float x[8];
@@ -433,9 +450,7 @@ block_read_kernel(const lq_block_kv c, const BlockSpan sp, T* __restrict__ k_out
   }
   for (int idx = tid; idx < rows * LPR; idx += kThreads) {
     const int pos = j * P + idx / LPR;
-    Pack8<T> r;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r.v[i] = Conv<T>::from_f32(0.f);
+    Pack8<T> r = zeros8<T>();
     if (pos < L) r = load8(ring + (int64_t)(pos % (2 * P)) * D + (idx % LPR) * 8, true);
     store8(out + (int64_t)idx * 8, r, true);
   }
