@@ -38,8 +38,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-__device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
-__device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
 // Bytes (sel) of biased codes (code + 128) under the high byte 0x64 are the halves 1024 + 128 + code.
 __device__ __forceinline__ uint32_t codes_h2(uint32_t biased, uint32_t sel) {
   return as_u32(__hsub2(as_h2(__byte_perm(biased, 0x64646464u, sel)), __floats2half2_rn(1152.f, 1152.f)));
@@ -193,16 +191,6 @@ __device__ __forceinline__ uint4 lds128m(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
-}
-template <typename T>
-__device__ __forceinline__ float2 pair_of(uint32_t v);
-template <>
-__device__ __forceinline__ float2 pair_of<__half>(uint32_t v) {
-  return __half22float2(as_h2(v));
-}
-template <>
-__device__ __forceinline__ float2 pair_of<__nv_bfloat16>(uint32_t v) {
-  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
 
 // ---------------------------------------------------------------- main kernel

@@ -53,19 +53,70 @@ __device__ __forceinline__ Pack8<T> zeros8() {
 }
 template <typename T>
 __device__ __forceinline__ void unpack8(const Pack8<T>& r, float (&x)[8]) {
-  T v[8];
-  memcpy(v, &r, sizeof(r));
+  const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = Conv<T>::to_f32(v[i]);
+  for (int i = 0; i < 4; ++i) {
+    const float2 p = pair_of<T>(w[i]);
+    x[2 * i] = p.x;
+    x[2 * i + 1] = p.y;
+  }
+}
+template <>
+__device__ __forceinline__ void unpack8<float>(const Pack8<float>& r, float (&x)[8]) {
+  const uint32_t w[8] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w, r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
 }
 template <typename T>
 __device__ __forceinline__ Pack8<T> pack8(const float (&x)[8]) {
-  T v[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = Conv<T>::from_f32(x[i]);
   Pack8<T> r;
-  memcpy(&r, v, sizeof(r));
+  r.w[0] = make_uint4(pair_to<T>(x[0], x[1]), pair_to<T>(x[2], x[3]), pair_to<T>(x[4], x[5]), pair_to<T>(x[6], x[7]));
   return r;
+}
+template <>
+__device__ __forceinline__ Pack8<float> pack8<float>(const float (&x)[8]) {
+  Pack8<float> r;
+  r.w[0] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  r.w[1] = make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7]));
+  return r;
+}
+
+// Two times four consecutive values (at elements a and b of a row)
+template <typename T>
+__device__ __forceinline__ Pack8<T> load44(const T* row, int a, int b, bool vec) {
+  Pack8<T> r;
+  if (vec) {
+    if (sizeof(T) == 2) {
+      const uint2 x = *reinterpret_cast<const uint2*>(row + a), y = *reinterpret_cast<const uint2*>(row + b);
+      r.w[0] = make_uint4(x.x, x.y, y.x, y.y);
+    } else {
+      r.w[0] = *reinterpret_cast<const uint4*>(row + a);
+      r.w[sizeof(T) / 2 - 1] = *reinterpret_cast<const uint4*>(row + b);
+    }
+  } else {
+    T v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] = row[a + i]; v[4 + i] = row[b + i]; }
+    memcpy(&r, v, sizeof(r));
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void store44(T* row, int a, int b, const Pack8<T>& r, bool vec) {
+  if (vec) {
+    if (sizeof(T) == 2) {
+      *reinterpret_cast<uint2*>(row + a) = make_uint2(r.w[0].x, r.w[0].y);
+      *reinterpret_cast<uint2*>(row + b) = make_uint2(r.w[0].z, r.w[0].w);
+    } else {
+      *reinterpret_cast<uint4*>(row + a) = r.w[0];
+      *reinterpret_cast<uint4*>(row + b) = r.w[sizeof(T) / 2 - 1];
+    }
+  } else {
+    T v[8];
+    memcpy(v, &r, sizeof(r));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { row[a + i] = v[i]; row[b + i] = v[4 + i]; }
+  }
 }
 
 // ---------------------------------------------------------------- norm + rotation of one head
@@ -78,42 +129,41 @@ struct Rope {
   float eps;
 };
 
-// This lane's 8 values' angles (values d0 .. d0 + 7 of the head), requested early.
-struct Angles {
-  float c[8], s[8];
+// The 8 values that lane li of a head's lanes holds: four from `a` on and four from `b` on, chosen so
+// that it has both values of each of its pairs and the rotation exchanges nothing between lanes.
+struct Hold {
+  int a, b;
 };
-__device__ __forceinline__ Angles angles_of(const Rope& rp, int64_t pos, int d0) {
-  Angles a;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) { a.c[i] = 1.f; a.s[i] = 0.f; }
-  if (d0 >= rp.rot) return a;
-  const int half = rp.rot / 2;
-  if (rp.interleaved) {
-    const float4 c = *reinterpret_cast<const float4*>(rp.cos + pos * half + d0 / 2);
-    const float4 s = *reinterpret_cast<const float4*>(rp.sin + pos * half + d0 / 2);
-    a.c[0] = a.c[1] = c.x; a.c[2] = a.c[3] = c.y; a.c[4] = a.c[5] = c.z; a.c[6] = a.c[7] = c.w;
-    a.s[0] = a.s[1] = s.x; a.s[2] = a.s[3] = s.y; a.s[4] = a.s[5] = s.z; a.s[6] = a.s[7] = s.w;
-  } else {
-    const int i0 = d0 < half ? d0 : d0 - half;
-    const float4* c = reinterpret_cast<const float4*>(rp.cos + pos * half + i0);
-    const float4* s = reinterpret_cast<const float4*>(rp.sin + pos * half + i0);
-    const float4 c0 = c[0], c1 = c[1], s0 = s[0], s1 = s[1];
-    a.c[0] = c0.x; a.c[1] = c0.y; a.c[2] = c0.z; a.c[3] = c0.w;
-    a.c[4] = c1.x; a.c[5] = c1.y; a.c[6] = c1.z; a.c[7] = c1.w;
-    a.s[0] = s0.x; a.s[1] = s0.y; a.s[2] = s0.z; a.s[3] = s0.w;
-    a.s[4] = s1.x; a.s[5] = s1.y; a.s[6] = s1.z; a.s[7] = s1.w;
+__device__ __forceinline__ Hold hold_of(int li, const Rope& rp) {
+  const bool halves = !rp.interleaved && li * 8 < rp.rot;
+  return halves ? Hold{li * 4, rp.rot / 2 + li * 4} : Hold{li * 8, li * 8 + 4};
+}
+
+// Cosines and sines of the lane's four pairs at a position (1 and 0 behind the rotated values).
+struct Angles {
+  float4 c, s;
+};
+__device__ __forceinline__ Angles angles_of(const Rope& rp, int64_t pos, int li) {
+  Angles a{make_float4(1.f, 1.f, 1.f, 1.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  if (li * 8 < rp.rot) {
+    a.c = *reinterpret_cast<const float4*>(rp.cos + pos * (rp.rot / 2) + li * 4);
+    a.s = *reinterpret_cast<const float4*>(rp.sin + pos * (rp.rot / 2) + li * 4);
   }
   return a;
 }
+// (p, q) -> (p cos - q sin, q cos + p sin)
+__device__ __forceinline__ void turn(float& p, float& q, float c, float s) {
+  const float x = __fmaf_rn(p, c, -__fmul_rn(q, s));
+  q = __fmaf_rn(q, c, __fmul_rn(p, s));
+  p = x;
+}
 
-// y = x * rsqrt(mean(x^2) + eps) * w over a head, then the rotation of its first rp.rot values:
-// pair (a, c) -> (a cos - c sin, c cos + a sin), a pair being (i, i + rot/2) or, interleaved,
-// (2i, 2i + 1). GRP lanes hold a head, 8 values each; all 32 lanes of the warp call this
-// together. fp32 throughout, every operation named, so that the joined and the separate forms
-// round alike; the caller rounds once.
+// y = x * rsqrt(mean(x^2) + eps) * w over a head, then the rotation of its first rp.rot values, a
+// pair being (i, i + rot/2) or, interleaved, (2i, 2i + 1). GRP lanes hold a head; all 32 lanes of
+// the warp call this together. fp32 throughout, every operation named, so that the joined and the
+// separate forms round alike; the caller rounds once.
 template <int GRP>
-__device__ __forceinline__ void norm_rope8(float (&x)[8], int li, int D, const float* w, const Rope& rp,
-                                           const Angles& a) {
+__device__ __forceinline__ void norm_rope8(float (&x)[8], int D, const float* w, const Rope& rp, const Angles& a) {
   if (w != nullptr) {
     float ss = 0.f;
 #pragma unroll
@@ -124,25 +174,16 @@ __device__ __forceinline__ void norm_rope8(float (&x)[8], int li, int D, const f
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], r), w[i]);
   }
-  const int d0 = li * 8;
   if (rp.interleaved) {
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const float p = x[i], q = x[i + 1];
-      x[i] = __fmaf_rn(p, a.c[i], -__fmul_rn(q, a.s[i]));
-      x[i + 1] = __fmaf_rn(q, a.c[i], __fmul_rn(p, a.s[i]));
-    }
+    turn(x[0], x[1], a.c.x, a.s.x);
+    turn(x[2], x[3], a.c.y, a.s.y);
+    turn(x[4], x[5], a.c.z, a.s.z);
+    turn(x[6], x[7], a.c.w, a.s.w);
   } else {
-    const int step = rp.rot / 16;  // lanes between the two values of a pair
-    const bool first = d0 < rp.rot / 2;
-    const int lane = threadIdx.x & 31;
-    const int src = d0 < rp.rot ? (first ? lane + step : lane - step) : lane;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float other = __shfl_sync(0xffffffffu, x[i], src);
-      const float turned = __fmul_rn(other, a.s[i]);  // (a.s is zero behind the rotated values)
-      x[i] = __fmaf_rn(x[i], a.c[i], first ? -turned : turned);
-    }
+    turn(x[0], x[4], a.c.x, a.s.x);
+    turn(x[1], x[5], a.c.y, a.s.y);
+    turn(x[2], x[6], a.c.z, a.s.z);
+    turn(x[3], x[7], a.c.w, a.s.w);
   }
 }
 
@@ -155,13 +196,13 @@ struct NormRopeArgs {
   int64_t ps[2];
   const T *q_weight, *k_weight;
   int B, T_new, Hq, Hk, D, heads_per_item, items_per_token;
-  int vec;
 };
 
 // A group of GRP lanes owns one token and up to heads_per_item of its heads: the token's angles
 // are loaded once and stay in registers. Bound by HBM (each value read and written once).
-template <typename T, int GRP>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const NormRopeArgs<T> p, const Rope rp, int* error_word) {
+template <typename T, int GRP, bool VEC>
+__global__ void __launch_bounds__(kThreads, 3)
+qk_norm_rope_kernel(const NormRopeArgs<T> p, const Rope rp, int* error_word) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int li = threadIdx.x % GRP;
@@ -170,59 +211,119 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const NormRopeAr
   const bool live = item0 < items;
   const int64_t item = live ? item0 : items - 1;
   const int64_t token = item / p.items_per_token;
-  const int chunk = (int)(item % p.items_per_token);
-  const int b = (int)(token / p.T_new), t = (int)(token % p.T_new);
+  const int chunk = (int)(item - token * p.items_per_token);
+  const int b = (int)(token / p.T_new), t = (int)(token - (int64_t)b * p.T_new);
   const int64_t at = p.positions[b * p.ps[0] + t * p.ps[1]];
   const bool known = at >= 0 && at < rp.table_len;
   if (!known && live && li == 0) atomicExch(error_word, LQ_BLOCK_BAD_ANGLE);
-  const int heads = p.Hq + p.Hk;
-  const int lo = chunk * p.heads_per_item, hi = min(lo + p.heads_per_item, heads);
+  const int lo = chunk * p.heads_per_item, hi = min(lo + p.heads_per_item, p.Hq + p.Hk);
   const bool mine = live && li * 8 < p.D;
-  const int d0 = mine ? li * 8 : 0;
-  const Angles a = angles_of(rp, known ? at : 0, li * 8 < p.D ? li * 8 : rp.rot);
-  constexpr int UN = 4;
+  const Hold own = mine ? hold_of(li, rp) : Hold{0, 4};
+  const Angles a = angles_of(rp, known ? at : 0, mine ? li : 32);
+  const T* q = p.q + b * p.qs[0] + t * p.qs[1];
+  const T* k = p.k + b * p.ks[0] + t * p.ks[1];
+  T* q_out = p.q_out + b * p.qos[0] + t * p.qos[1];
+  T* k_out = p.k_out + b * p.kos[0] + t * p.kos[1];
+  constexpr int UN = 4;  // heads on their way at once
   float w[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   int held = -1;  // whose weights are in w: 0 queries', 1 keys'
+#pragma unroll 1
   for (int h0 = lo; h0 < lo + p.heads_per_item; h0 += UN) {  // (the same trip count for the whole warp)
     Pack8<T> in[UN];
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       const int h = h0 + u;
-      if (mine && h < hi) {
-        const T* src = h < p.Hq ? p.q + b * p.qs[0] + t * p.qs[1] + h * p.qs[2]
-                                : p.k + b * p.ks[0] + t * p.ks[1] + (h - p.Hq) * p.ks[2];
-        in[u] = load8(src + d0, p.vec);
-      } else {
-        in[u] = zeros8<T>();
-      }
+      in[u] = zeros8<T>();
+      if (mine && h < hi) in[u] = load44(h < p.Hq ? q + h * p.qs[2] : k + (h - p.Hq) * p.ks[2], own.a, own.b, VEC);
     }
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       const int h = h0 + u;
-      if (u > 0 && u >= p.heads_per_item) break;
+      if (u >= p.heads_per_item) break;
       const int whose = h < p.Hq ? 0 : 1;
-      const T* weight = whose ? p.k_weight : p.q_weight;
-      if (p.q_weight != nullptr && whose != held && mine && h < hi) {
-        unpack8(load8(weight + d0, p.vec), w);
+      if (p.q_weight != nullptr && whose != held && mine) {
+        unpack8(load44(whose ? p.k_weight : p.q_weight, own.a, own.b, VEC), w);
         held = whose;
       }
       float x[8];
       unpack8(in[u], x);
-      norm_rope8<GRP>(x, li, p.D, p.q_weight != nullptr ? w : nullptr, rp, a);
+      norm_rope8<GRP>(x, p.D, p.q_weight != nullptr ? w : nullptr, rp, a);
       if (mine && h < hi) {
         if (!known) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] = __int_as_float(0x7fffffff);  // no angle: nothing usable
         }
-        T* dst = h < p.Hq ? p.q_out + b * p.qos[0] + t * p.qos[1] + h * p.qos[2]
-                          : p.k_out + b * p.kos[0] + t * p.kos[1] + (h - p.Hq) * p.kos[2];
-        store8(dst + d0, pack8<T>(x), p.vec);
+        store44(h < p.Hq ? q_out + h * p.qos[2] : k_out + (h - p.Hq) * p.kos[2], own.a, own.b, pack8<T>(x), VEC);
       }
     }
   }
 }
 
 // ---------------------------------------------------------------- append
+// The largest magnitude of what a thread holds, INF if any of it is not finite. 16-bit values are
+// compared as pairs (the comparison keeps NaN).
+template <typename T>
+struct Largest {
+  float top = 0.f;
+  __device__ __forceinline__ void take(const Pack8<T>& r) {
+    float x[8];
+    unpack8(r, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float m = fabsf(x[i]);
+      top = m <= 3.402823466e38f ? fmaxf(top, m) : INFINITY;
+    }
+  }
+  __device__ __forceinline__ float value() const { return top; }
+};
+template <typename T2>
+struct LargestPair {
+  T2 top;
+  __device__ __forceinline__ LargestPair() { memset(&top, 0, sizeof(top)); }
+  template <typename P>
+  __device__ __forceinline__ void take(const P& r) {
+    const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const T2*>(&w[i])));
+  }
+  __device__ __forceinline__ float value(float lo, float hi) const {
+    const float m = fmaxf(lo, hi);
+    return lo <= 3.402823466e38f && hi <= 3.402823466e38f ? m : INFINITY;
+  }
+};
+template <>
+struct Largest<__half> : LargestPair<__half2> {
+  __device__ __forceinline__ float value() const { return LargestPair::value(__low2float(top), __high2float(top)); }
+};
+template <>
+struct Largest<__nv_bfloat16> : LargestPair<__nv_bfloat162> {
+  __device__ __forceinline__ float value() const { return LargestPair::value(__low2float(top), __high2float(top)); }
+};
+
+// Codes of 8 values: rint(x / scale) with IEEE division. x * (1 / scale) is within 2e-5 of the quotient
+// (magnitudes up to 127, three roundings of 2^-24), so its rounding is the quotient's unless it lies
+// that near to a half; then, one value in some thousands, the division itself decides. Adding
+// 1.5 * 2^23 rounds to the nearest even integer and leaves it in the low byte. |x| <= 127 scale
+// up to rounding, so there is nothing to clamp.
+__device__ __forceinline__ uint2 codes8(const float (&x)[8], float scale, float inv) {
+  constexpr float kMagic = 12582912.f;
+  uint32_t q[8];
+  float worst = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float r = __fmaf_rn(x[i], inv, kMagic);
+    q[i] = __float_as_uint(r);
+    worst = fmaxf(worst, fabsf(__fmaf_rn(x[i], inv, -__fsub_rn(r, kMagic))));
+  }
+  if (worst > 0.4998f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = (uint32_t)(int)code_of(x[i], scale, -128.f, 127.f);
+  }
+  const uint32_t lo = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+  const uint32_t hi = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
+  return make_uint2(lo, hi);
+}
+
 template <typename T>
 struct AppendArgs {
   const T *k, *v;            // plain form: new rows
@@ -243,7 +344,7 @@ struct AppendArgs {
 // a later block of the same parity replaces; its CTA then writes that later block's rows too,
 // after its own reads.
 template <typename T, int D, bool JOINED>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2)
 block_append_kernel(const lq_block_kv c, const BlockSpan sp, const AppendArgs<T> p, const Rope rp, int* error_word) {
   constexpr int LPR = D / 8;  // lanes that hold a row
   __shared__ float red[kThreads / 32];
@@ -262,7 +363,8 @@ block_append_kernel(const lq_block_kv c, const BlockSpan sp, const AppendArgs<T>
   const bool query_cta = JOINED && (int)blockIdx.y >= 2 * c.kv_heads;
   const bool is_v = blockIdx.y & 1;
   const T* weight = !JOINED ? nullptr : (query_cta ? p.q_weight : p.k_weight);
-  if (JOINED && weight != nullptr) unpack8(load8(weight + li * 8, p.vec), w);
+  const Hold own = JOINED && (query_cta || !is_v) ? hold_of(li, rp) : Hold{li * 8, li * 8 + 4};
+  if (JOINED && weight != nullptr) unpack8(load44(weight, own.a, own.b, p.vec), w);
 
   if (query_cta) {
     const int rows = sp.tokens * p.Hq;
@@ -276,9 +378,9 @@ block_append_kernel(const lq_block_kv c, const BlockSpan sp, const AppendArgs<T>
       const int64_t pos = s.start + t;
       const bool known = pos < rp.table_len;
       float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (fresh) unpack8(load8(p.q + b * p.qs[0] + h * p.qs[1] + t * p.qs[2] + li * 8, p.vec), x);
-      const Angles a = angles_of(rp, fresh && known ? pos : 0, li * 8);
-      norm_rope8<LPR>(x, li, D, weight != nullptr ? w : nullptr, rp, a);
+      if (fresh) unpack8(load44(p.q + b * p.qs[0] + h * p.qs[1] + t * p.qs[2], own.a, own.b, p.vec), x);
+      const Angles a = angles_of(rp, fresh && known ? pos : 0, li);
+      norm_rope8<LPR>(x, D, weight != nullptr ? w : nullptr, rp, a);
       if (fresh && !known) {
         if (li == 0) atomicExch(error_word, LQ_BLOCK_BAD_ANGLE);
 #pragma unroll
@@ -289,7 +391,7 @@ block_append_kernel(const lq_block_kv c, const BlockSpan sp, const AppendArgs<T>
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] = 0.f;  // rows behind the sequence's count
         }
-        store8(p.q_out + (((int64_t)b * sp.tokens + t) * p.Hq + h) * D + li * 8, pack8<T>(x), true);
+        store44(p.q_out + (((int64_t)b * sp.tokens + t) * p.Hq + h) * D, own.a, own.b, pack8<T>(x), true);
       }
     }
     return;
@@ -306,16 +408,22 @@ block_append_kernel(const lq_block_kv c, const BlockSpan sp, const AppendArgs<T>
   const int64_t step = is_v ? p.vs[2] : p.ks[2];
   const bool turned = JOINED && !is_v;
 
-  // one 8-value piece of a new row; every lane of the warp calls it
+  // this thread's 8 values of a row
+  auto row_load = [&](const T* row, bool vec) { return JOINED ? load44(row, own.a, own.b, vec) : load8(row + li * 8, vec); };
+  auto row_store = [&](T* row, const Pack8<T>& r) {
+    if (JOINED) store44(row, own.a, own.b, r, true);
+    else store8(row + li * 8, r, true);
+  };
+  // the same of a new row; every lane of the warp calls it
   auto fetch = [&](int pos, bool fresh) {
     Pack8<T> r = zeros8<T>();
-    if (fresh) r = load8(src + (int64_t)(pos - s.start) * step + li * 8, p.vec);
+    if (fresh) r = row_load(src + (int64_t)(pos - s.start) * step, p.vec);
     if (turned) {
       float x[8];
       unpack8(r, x);
       const bool known = pos < rp.table_len;
-      const Angles a = angles_of(rp, fresh && known ? pos : 0, li * 8);
-      norm_rope8<LPR>(x, li, D, weight != nullptr ? w : nullptr, rp, a);
+      const Angles a = angles_of(rp, fresh && known ? pos : 0, li);
+      norm_rope8<LPR>(x, D, weight != nullptr ? w : nullptr, rp, a);
       if (fresh && !known) {
         if (li == 0) atomicExch(error_word, LQ_BLOCK_BAD_ANGLE);
 #pragma unroll
@@ -329,7 +437,7 @@ block_append_kernel(const lq_block_kv c, const BlockSpan sp, const AppendArgs<T>
   const bool to_ring = j >= last - 1 && !(reads_ring && j != first && ((j ^ first) & 1) == 0);
   const int pieces = P * LPR;
   Pack8<T> val[kMaxVec];
-  float amax = 0.f;
+  Largest<T> top;
 #pragma unroll
   for (int v = 0; v < kMaxVec; ++v) {
     if (v * kThreads < pieces) {
@@ -337,22 +445,15 @@ block_append_kernel(const lq_block_kv c, const BlockSpan sp, const AppendArgs<T>
       const int row = idx / LPR, pos = j * P + row;
       const bool inside = idx < pieces;
       const bool fresh = inside && pos >= s.start && pos < L;
+      T* held = ring + (int64_t)(pos & (2 * P - 1)) * D;
       val[v] = fetch(pos, fresh);
-      if (inside && complete && pos < s.start) val[v] = load8(ring + (int64_t)(pos % (2 * P)) * D + li * 8, true);
-      if (fresh && to_ring) store8(ring + (int64_t)(pos % (2 * P)) * D + li * 8, val[v], true);
-      if (complete) {
-        float x[8];
-        unpack8(val[v], x);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float m = fabsf(x[i]);
-          amax = m <= 3.402823466e38f ? fmaxf(amax, m) : INFINITY;  // INF and NaN both: not finite
-        }
-      }
+      if (inside && complete && pos < s.start) val[v] = row_load(held, true);
+      if (fresh && to_ring) row_store(held, val[v]);
+      if (complete) top.take(val[v]);
     }
   }
   if (!complete) return;
-  amax = warp_max(amax);
+  float amax = warp_max(top.value());
   if ((tid & 31) == 0) red[tid >> 5] = amax;
   __syncthreads();  // (also: every read of the ring above is done)
   amax = red[0];
@@ -360,6 +461,7 @@ block_append_kernel(const lq_block_kv c, const BlockSpan sp, const AppendArgs<T>
   for (int i = 1; i < kThreads / 32; ++i) amax = fmaxf(amax, red[i]);
   const bool finite = amax <= 3.402823466e38f;
   const float scale = finite ? scale_of(amax, 127.f) : __int_as_float(0x7fffffff);
+  const float inv = finite ? __fdiv_rn(1.f, scale) : 0.f;
   const int64_t page = page_of(c, b, j);
   if (page < 0) {
     if (tid == 0) atomicExch(error_word, LQ_BLOCK_BAD_PAGE);
@@ -373,10 +475,14 @@ block_append_kernel(const lq_block_kv c, const BlockSpan sp, const AppendArgs<T>
       if (idx < pieces) {
         float x[8];
         unpack8(val[v], x);
-        alignas(8) int8_t q[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = finite ? (int8_t)code_of(x[i], scale, -128.f, 127.f) : (int8_t)0;
-        *reinterpret_cast<uint2*>(codes + (int64_t)idx * 8) = *reinterpret_cast<const uint2*>(q);
+        const uint2 q = finite ? codes8(x, scale, inv) : make_uint2(0u, 0u);
+        if (JOINED) {
+          int8_t* row = codes + (int64_t)(idx / LPR) * D;
+          *reinterpret_cast<uint32_t*>(row + own.a) = q.x;
+          *reinterpret_cast<uint32_t*>(row + own.b) = q.y;
+        } else {
+          *reinterpret_cast<uint2*>(codes + (int64_t)idx * 8) = q;
+        }
       }
     }
   }
@@ -388,7 +494,7 @@ block_append_kernel(const lq_block_kv c, const BlockSpan sp, const AppendArgs<T>
         const int pos = jx * P + idx / LPR;
         const bool fresh = idx < pieces && pos < L;
         const Pack8<T> r = fetch(pos, fresh);
-        if (fresh) store8(ring + (int64_t)(pos % (2 * P)) * D + li * 8, r, true);
+        if (fresh) row_store(ring + (int64_t)(pos & (2 * P - 1)) * D, r);
       }
     }
   }
@@ -451,7 +557,7 @@ block_read_kernel(const lq_block_kv c, const BlockSpan sp, T* __restrict__ k_out
   for (int idx = tid; idx < rows * LPR; idx += kThreads) {
     const int pos = j * P + idx / LPR;
     Pack8<T> r = zeros8<T>();
-    if (pos < L) r = load8(ring + (int64_t)(pos % (2 * P)) * D + (idx % LPR) * 8, true);
+    if (pos < L) r = load8(ring + (int64_t)(pos & (2 * P - 1)) * D + (idx % LPR) * 8, true);
     store8(out + (int64_t)idx * 8, r, true);
   }
 }
@@ -596,6 +702,10 @@ extern "C" int lq_qk_norm_rope(const void* q, const void* k, const int64_t* q_st
   const int64_t groups = (int64_t)B * T_new * items_per_token;
   const int64_t ctas = (groups + kThreads / grp - 1) / (kThreads / grp);
   LQ_REQUIRE(ctas <= 0x7fffffffLL, LQ_ERR_ARG, "too many rows for one launch");
+#define LQ_GRP(G)                                                                             \
+  if (grp == G)                                                                               \
+    return vec ? launch(qk_norm_rope_kernel<T, G, true>, grid, s, pdl, what, p, rp, error_word) \
+               : launch(qk_norm_rope_kernel<T, G, false>, grid, s, pdl, what, p, rp, error_word);
   LQ_DISPATCH_DTYPE(dtype, T, {
     NormRopeArgs<T> p;
     p.q = (const T*)q; p.k = (const T*)k; p.q_out = (T*)q_out; p.k_out = (T*)k_out;
@@ -610,17 +720,13 @@ extern "C" int lq_qk_norm_rope(const void* q, const void* k, const int64_t* q_st
     p.positions = positions; p.ps[0] = pos_stride_b; p.ps[1] = pos_stride_t;
     p.q_weight = (const T*)(Hq ? q_weight : k_weight); p.k_weight = (const T*)k_weight;
     p.B = B; p.T_new = T_new; p.Hq = Hq; p.Hk = Hk; p.D = D;
-    p.heads_per_item = per; p.items_per_token = items_per_token; p.vec = vec;
+    p.heads_per_item = per; p.items_per_token = items_per_token;
     const dim3 grid((unsigned)ctas);
     const cudaStream_t s = (cudaStream_t)stream;
     const char* what = "lq_qk_norm_rope";
-    switch (grp) {
-      case 4: return launch(qk_norm_rope_kernel<T, 4>, grid, s, pdl, what, p, rp, error_word);
-      case 8: return launch(qk_norm_rope_kernel<T, 8>, grid, s, pdl, what, p, rp, error_word);
-      case 16: return launch(qk_norm_rope_kernel<T, 16>, grid, s, pdl, what, p, rp, error_word);
-      default: return launch(qk_norm_rope_kernel<T, 32>, grid, s, pdl, what, p, rp, error_word);
-    }
+    LQ_GRP(4) LQ_GRP(8) LQ_GRP(16) LQ_GRP(32)
   })
+#undef LQ_GRP
   return LQ_OK;
 }
 

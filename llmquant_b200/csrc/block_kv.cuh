@@ -47,6 +47,31 @@ __device__ __forceinline__ int64_t page_of(const lq_block_kv& c, int b, int j) {
   return id >= 0 && id < c.num_pages ? id : -1;
 }
 
+// Two 16-bit values in a word, to and from fp32
+__device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+__device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+template <typename T>
+__device__ __forceinline__ float2 pair_of(uint32_t v);
+template <>
+__device__ __forceinline__ float2 pair_of<__half>(uint32_t v) {
+  return __half22float2(as_h2(v));
+}
+template <>
+__device__ __forceinline__ float2 pair_of<__nv_bfloat16>(uint32_t v) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pair_to(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pair_to<__half>(float lo, float hi) {
+  return as_u32(__floats2half2_rn(lo, hi));
+}
+template <>
+__device__ __forceinline__ uint32_t pair_to<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 // Address of the current device's error word (NULL and a message if it cannot be resolved).
 int* block_error_word();
 // Host checks shared by every entry point that takes a cache.
