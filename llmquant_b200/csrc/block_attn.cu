@@ -9,28 +9,37 @@
 //   O  += w_p code_p,  sum += (sum of the block's w_p) / vs,   out = O / sum.
 //
 // A unit of work is 32 tokens of one KV head. The units of all sequences and heads form one line,
-// which the CTAs share in equal contiguous runs, so ragged lengths and single long contexts both
-// fill the GPU without the host knowing a length. A CTA's warps take the units of its run in
-// turn; at the end of a (sequence, head) they merge through shared memory, and where a run ends
-// inside one the partial (M, sum, O) goes to scratch and the second kernel joins the parts.
+// which the warps share in contiguous runs, so ragged lengths and single long contexts both fill
+// the GPU without the host knowing a length. A warp is a CTA: it never waits for another one. At
+// the end of a (sequence, head), or of its run, it writes the outputs where it had all of it, else a
+// partial (M, sum, O) to scratch, and the second kernel joins the parts.
 //
 // Scores are computed as K q^T (16 tokens x 8 query rows a tile) and outputs as V^T w (16 dims x 8
 // query rows), so that the few query rows of a decode step are the narrow side of the MMA: with
 // queries as its 16 rows half of every product would be padding. The k index of the first product
 // and the row index of the second are mapped onto the head's dims so that each thread's bytes of
 // a cached row are contiguous.
+#include <type_traits>
+
 #include "block_kv.cuh"
 
 namespace lq {
 namespace {
 
 constexpr int kUnit = 32;  // tokens, as two halves of 16 (the height of an MMA tile)
+constexpr float kNone = -1e30f;  // a maximum of nothing: below any score, and 2^(kNone - M) is zero
 
 __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                       uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
@@ -61,6 +70,11 @@ __device__ __forceinline__ float exp2_of(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float log2_of(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float inverse_of(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -68,10 +82,19 @@ __device__ __forceinline__ float inverse_of(float x) {
 }
 
 // ---------------------------------------------------------------- how the line of units is cut
+#ifndef LQ_S0
+#define LQ_S0 80
+#endif
+constexpr int kFirst = LQ_S0;  // per cent of a long line that the warps which run at once take
+
 struct Shape {
   int Hq, G, rows, tile;  // query rows per KV head: T_new * G; rows of one pass
-  int warps;              // of a CTA of the main kernel
+  uint64_t inv_G;         // ceil(2^32 / G): (row * inv_G) >> 32 = row / G for row * G < 2^32
+  int slots, waves;       // warps of a tile's line that run at once; 2: a second wave for long lines
+  uint32_t step;          // 2^32 / slots
 };
+
+__device__ __forceinline__ int token_of(const Shape& sh, int row) { return (int)((uint64_t)(unsigned)row * sh.inv_G >> 32); }
 
 // The tokens row tile rt of sequence b is about.
 struct Tile {
@@ -83,9 +106,9 @@ struct Tile {
 __device__ __forceinline__ Tile tile_of(const lq_block_kv& c, const BlockSpan& sp, const Shape& sh, int b, int rt) {
   Tile x;
   x.s = span_of(c, sp, b, x.bad);
-  x.t_lo = rt * sh.tile / sh.G;
+  x.t_lo = token_of(sh, rt * sh.tile);
   const int L = x.s.start + x.s.n;
-  x.visible = x.s.start + min(x.s.n, (rt * sh.tile + sh.tile - 1) / sh.G + 1);
+  x.visible = x.s.start + min(x.s.n, token_of(sh, rt * sh.tile + sh.tile - 1) + 1);
   x.held = L & ~(c.block - 1);
   x.code_units = (min(x.visible, x.held) + kUnit - 1) / kUnit;
   x.units = x.code_units + (max(0, x.visible - x.held) + kUnit - 1) / kUnit;
@@ -93,25 +116,34 @@ __device__ __forceinline__ Tile tile_of(const lq_block_kv& c, const BlockSpan& s
   return x;
 }
 
-// The line of `total` units is shared by n CTAs: n no larger than one for each round of a CTA's warps,
-// but one for each (sequence, head) where those are more, so that short contexts need no join. The
-// first `rem` CTAs take base + 1 units, the others base.
+// How the warps share the line of `total` units: up to one unit for each warp that runs at once, one
+// each; up to eight, equal runs; above, with one row tile, equal runs over kFirst per cent and as many
+// short ones over the rest: SMs stream at speeds up to 30 % apart, and the short runs go to those
+// that are done first. (Multiplications in place of divisions: every warp begins with this.)
 struct Cut {
-  int total, n, base, rem;
-  __device__ __forceinline__ int begin(int cta) const { return cta * base + min(cta, rem); }
-  __device__ __forceinline__ int owner(int unit) const {
-    const int wide = rem * (base + 1);
-    return unit < wide ? unit / (base + 1) : rem + (unit - wide) / base;
+  int total, first;  // units of the first wave
+  int kind;
+  __device__ __forceinline__ Cut(int total_, const Shape& sh) : total(total_), first(total_) {
+    kind = total <= sh.slots ? 0 : (sh.waves == 1 || total <= 8 * sh.slots) ? 1 : 2;
+    if (kind == 2) first = (int)((int64_t)total * (0x100000000LL / 100 * kFirst) >> 32);
+  }
+  __device__ __forceinline__ int begin(const Shape& sh, int i) const {
+    if (kind == 0) return min(i, total);
+    if (i < sh.slots) return (int)((uint64_t)first * ((uint64_t)sh.step * i) >> 32);
+    if (kind == 1 || i >= 2 * sh.slots) return total;
+    return first + (int)((uint64_t)(total - first) * ((uint64_t)sh.step * (i - sh.slots)) >> 32);
+  }
+  __device__ __forceinline__ int owner(const Shape& sh, int unit) const {  // begin(owner) <= unit < begin(owner + 1)
+    if (kind == 0) return unit;
+    const bool later = unit >= first;
+    const int wave = later ? sh.slots : 0, last = later ? 2 * sh.slots - 1 : sh.slots - 1;
+    const float per = (float)sh.slots / (float)(later ? total - first : first);
+    int i = min(last, wave + (int)((float)(unit - (later ? first : 0)) * per));
+    while (begin(sh, i) > unit) --i;
+    while (i < last && begin(sh, i + 1) <= unit) ++i;
+    return i;
   }
 };
-__device__ __forceinline__ Cut cut_of(int total, int ctas, int heads, int warps) {
-  Cut k;
-  k.total = total;
-  k.n = min(min(ctas, total), max((total + warps - 1) / warps, heads));
-  k.base = k.n > 0 ? total / k.n : 0;
-  k.rem = total - k.n * k.base;
-  return k;
-}
 
 // All units of row tile rt and, of those, the ones before sequence `b`. One warp calls it.
 __device__ __forceinline__ int2 units_before(const lq_block_kv& c, const BlockSpan& sp, const Shape& sh, int rt, int b) {
@@ -126,54 +158,54 @@ __device__ __forceinline__ int2 units_before(const lq_block_kv& c, const BlockSp
   return make_int2(total * c.kv_heads, before * c.kv_heads);
 }
 
-// The sequence that unit `unit` of the line lies in, and the units before that sequence.
-__device__ __forceinline__ int2 sequence_of(const lq_block_kv& c, const BlockSpan& sp, const Shape& sh, int rt, int unit) {
+// Where run `run` of the line lies: its length, its first sequence, and its begin behind that
+// sequence's. One warp calls it.
+__device__ __forceinline__ int3 run_of(const lq_block_kv& c, const BlockSpan& sp, const Shape& sh, int rt, int run) {
   const int lane = threadIdx.x & 31;
+  int total = 0, mine = 0;
+  for (int i = lane; i < c.batch; i += 32) total += mine = tile_of(c, sp, sh, i, rt).units * c.kv_heads;
+  total = __reduce_add_sync(0xffffffffu, total);
+  const Cut cut(total, sh);
+  const int begin = cut.begin(sh, run), length = cut.begin(sh, run + 1) - begin;
   int before = 0;
   for (int b0 = 0; b0 < c.batch; b0 += 32) {
-    const int mine = b0 + lane < c.batch ? tile_of(c, sp, sh, b0 + lane, rt).units * c.kv_heads : 0;
+    if (c.batch > 32) mine = b0 + lane < c.batch ? tile_of(c, sp, sh, b0 + lane, rt).units * c.kv_heads : 0;
     int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += v;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + upto > unit);
+    const unsigned hit = __ballot_sync(0xffffffffu, before + upto > begin);
     if (hit != 0) {
       const int at = __ffs(hit) - 1;
-      return make_int2(b0 + at, before + __shfl_sync(0xffffffffu, upto - mine, at));
+      return make_int3(length, b0 + at, begin - before - __shfl_sync(0xffffffffu, upto - mine, at));
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
   }
-  return make_int2(c.batch, before);
+  return make_int3(0, c.batch, 0);
 }
 
-// NT: groups of 8 query rows of a pass. What bounds the choice: the outputs take NT * D / 4
-// registers of a thread. One group: 12 warps of 168 registers; two: 8 warps of 255.
+// NT: groups of 8 query rows of a pass. The outputs take NT * D / 4 registers of a thread, so an SM holds 12
+// warps with one group and 8 with two; their rings fill its shared memory.
 template <int D, int NT>
 struct Cfg {
-  static constexpr int kWarps = NT == 1 ? 12 : 8;
-  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kWarps = NT == 1 ? 12 : 8;        // on an SM
   static constexpr int kRows = 8 * NT;
-  static constexpr int kHalf = 16 * D;                   // bytes of 16 tokens' keys, or values
-  static constexpr int kStage = 4 * kHalf + 16;          // K and V of half 0, of half 1, their scales
+  static constexpr int kCodes = kUnit * D;               // bytes of a unit's keys, or values
+  static constexpr int kStage = 2 * kCodes + 16;         // keys, values, (key, value) scales of the two halves
   static constexpr int kStages = (NT == 1 ? 2 : 3) * (128 / D);  // units in a warp's ring
-  static constexpr int kQ = D + 4;                       // halves to a staged query row: rows 8 bytes apart in the banks
-  static constexpr int kO = D + 4;                       // floats to a partial output row
-  static constexpr int kWarpBytes = kStages * kStage;    // also a warp's partial outputs, once the ring is drained
-  static constexpr size_t kQBytes = (size_t)kRows * kQ * 2;
-  static constexpr size_t kMlBytes = (size_t)kWarps * kRows * 8;
-  static constexpr size_t kTotal = (size_t)kWarps * kWarpBytes + kQBytes + kMlBytes + kRows * 4;
-  static_assert(kWarpBytes % 16 == 0 && kQBytes % 8 == 0 && kRows * kO * 4 <= kWarpBytes && kTotal <= 227 * 1024, "");
+  static constexpr size_t kRing = kStages * kStage;
+  static_assert(kStage % 16 == 0 && kWarps * (kRing + 1024) <= 228 * 1024, "");
 };
 
-// 16-byte piece `chunk` of row `row` of 16 staged tokens. Pieces are XOR-swizzled so that both readers
-// are free of bank conflicts: the score product's threads (8 rows, pieces 2 q4 + j) and the value
-// product's (rows 2 q4, piece gid).
+// Offset of 16-byte piece `chunk` of row `row` of a unit's staged keys or values. Pieces are
+// XOR-swizzled so that both readers are free of bank conflicts: the score product's threads (8 rows
+// gid, pieces 2 q4 + j) and the value product's (rows 2 q4, piece gid).
 template <int D>
 __device__ __forceinline__ uint32_t piece_at(int row, int chunk) {
   if (D == 128) return (uint32_t)row * 128 + ((chunk ^ (row & 7)) << 4);
-  return (uint32_t)(row >> 1) * 128 + (((((row & 1) << 2) + chunk) ^ ((row & 6))) << 4);
+  return (uint32_t)(row >> 1) * 128 + (((((row & 1) << 2) + chunk) ^ (row & 6)) << 4);
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -193,49 +225,62 @@ __device__ __forceinline__ uint4 lds128m(uint32_t addr) {
   return v;
 }
 
+// 16 * J consecutive values of a 16-bit row as words
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint16_t* p, bool there, int vec) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) w[i] = 0u;
+  if (!there) return;
+  if (vec) {  // on a 16-byte boundary
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+  }
+}
+
 // ---------------------------------------------------------------- main kernel
-// grid (CTAs that share the line, row tiles). T is the type of q, out and the ring.
+// grid (runs of the line, row tiles), one warp. T is the type of q, out and the ring.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__((Cfg<D, NT>::kThreads), 1)
+__global__ void __launch_bounds__(32, (Cfg<D, NT>::kWarps))
 block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const T* __restrict__ q, int64_t qsb, int64_t qst,
-                  int64_t qsh, T* __restrict__ out, float* __restrict__ part, float2* __restrict__ part_ml, float qk_scale,
-                  int* error_word) {
+                  int64_t qsh, int q_vec, T* __restrict__ out, float* __restrict__ part, float2* __restrict__ part_ml,
+                  float qk_scale, int* error_word) {
   using C = Cfg<D, NT>;
-  constexpr int W = C::kWarps, ROWS = C::kRows, KS = D / 16, MT = D / 16, DPT = D / 8;  // DPT: dims of V a thread owns
+  constexpr int ROWS = C::kRows, KS = D / 16, MT = D / 16, DPT = D / 8;  // DPT: dims of V a thread owns
   constexpr int J = D / 64;  // 16-byte pieces of a K row a thread reads
-  extern __shared__ __align__(16) uint8_t smem[];
-  __half* q_s = reinterpret_cast<__half*>(smem + (size_t)W * C::kWarpBytes);
-  float2* ml_s = reinterpret_cast<float2*>(smem + (size_t)W * C::kWarpBytes + C::kQBytes);
-  float* unit_s = reinterpret_cast<float*>(smem + (size_t)W * C::kWarpBytes + C::kQBytes + C::kMlBytes);
-  __shared__ int line_s[3];
+  extern __shared__ __align__(16) uint8_t ring[];
+  // One group of bf16 queries meets the codes as 15-bit integers in two byte planes: the codes then need
+  // no conversion. fp16 queries keep their 11 bits as fp16; with more groups the conversion is shared
+  // and the integer product's lower rate counts (chunk of 512: 278 us by integers, 242 by fp16).
+  constexpr bool kInt = NT == 1 && std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kTop = kInt ? 13 : 10;  // exponent that a row's largest value is lifted to
 
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int gid = lane >> 2, q4 = lane & 3;
+  const int lane = threadIdx.x, gid = lane >> 2, q4 = lane & 3;
   const int rt = blockIdx.y, P = c.block, shift = 31 - __clz(P);
-  const int cta = blockIdx.x, heads = c.batch * c.kv_heads;
-  if (warp == 0) {
-    const int total = units_before(c, sp, sh, rt, 0).x;
-    const Cut cut = cut_of(total, gridDim.x, heads, W);
-    const int2 at = sequence_of(c, sp, sh, rt, cta < cut.n ? cut.begin(cta) : total);
-    if (lane == 0) {
-      line_s[0] = total;
-      line_s[1] = at.x;
-      line_s[2] = at.y;
-    }
-  }
-  __syncthreads();
-  const Cut cut = cut_of(line_s[0], gridDim.x, heads, W);
-  if (cta >= cut.n) return;
-  int left = cut.begin(cta + 1) - cut.begin(cta);
-  int off = cut.begin(cta) - line_s[2];
-  uint8_t* ring = smem + (size_t)warp * C::kWarpBytes;
+  const int heads = c.batch * c.kv_heads;
+  const int3 run = run_of(c, sp, sh, rt, blockIdx.x);
+  int left = run.x, off = run.z;  // units of this run; where it begins behind its first sequence
   const uint32_t ring_a = smem_u32(ring);
+  // this lane's places in a stage: pieces it copies (the i-th at + 512 i, alternating at D = 128), pieces of
+  // K it reads (rows gid + 8 e at + 8 D e), pieces of V (rows 2 q4 + 8 e at + 8 D e)
+  const uint32_t copy_at = piece_at<D>(lane / (D / 16), lane % (D / 16));
+  uint32_t k_at[J], v_at[2];
+#pragma unroll
+  for (int j = 0; j < J; ++j) k_at[j] = piece_at<D>(gid, q4 * J + j);
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    v_at[k] = C::kCodes + (D == 128 ? piece_at<D>(q4 * 2 + k, gid) : piece_at<D>(q4 * 2 + k, gid >> 1) + (gid & 1) * 8);
 
 #pragma unroll 1
-  for (int b = line_s[1]; left > 0 && b < c.batch; ++b) {
+  for (int b = run.y; left > 0; ++b) {
     const Tile x = tile_of(c, sp, sh, b, rt);
     if (off >= x.units * c.kv_heads) {
       off -= x.units * c.kv_heads;
@@ -250,95 +295,121 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
       off += ub - ua;
       left -= ub - ua;
 
-      // ---- the warp's ring: codes and scales of its units, kStages - 1 of them on their way. The page
-      // ids of a unit are requested one unit earlier than its codes.
+      // ---- the ring: codes and scales of the next units, kStages - 1 of them on their way. The page ids
+      // of a unit are requested one unit earlier than its codes.
       const int last_code = min(ub, x.code_units);
       const int code_end = min(x.visible, x.held);
-      int ids[2];
       auto look_up = [&](int u) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int pos = u * kUnit + 16 * e;
-          ids[e] = u < last_code && pos < code_end ? table[pos >> shift] : 0;
-        }
+        const int pos = u * kUnit;
+        return make_int2(u < last_code ? table[pos >> shift] : 0,
+                         P == 16 && u < last_code && pos + 16 < code_end ? table[(pos >> 4) + 1] : 0);
       };
-      auto issue = [&](int u, int stage) {
+      // `halves` times 16 tokens of a page, from row `first` of it on, to half e of a stage
+      auto copy = [&](int id, int first, int e, int stage, auto halves) {
+        const uint32_t dst = ring_a + stage * C::kStage + e * (C::kCodes / 2);
+        const uint32_t scale_dst = ring_a + stage * C::kStage + 2 * C::kCodes + e * 8;
+        if (id < 0 || id >= c.num_pages) {
+          if (lane == 0) atomicExch(error_word, LQ_BLOCK_BAD_PAGE);
+          if (lane < 2 * halves) asm volatile("st.shared.u32 [%0], %1;" ::"r"(scale_dst + lane * 4), "r"(0x7fffffff) : "memory");
+          return;
+        }
+        const int ph = id * c.kv_heads + h;  // (pages * heads fit 31 bits: a page takes over 2 kB)
+        const int64_t at = (((int64_t)ph << shift) + first) * D + lane * 16;
+        const int8_t* kp = c.k_pages + at;
+        const int8_t* vp = c.v_pages + at;
+#pragma unroll
+        for (int i = 0; i < halves * D / 32; ++i) {
+          const uint32_t to = dst + i * 512 + (D == 128 && (i & 1) ? copy_at ^ 64u : copy_at);
+          cp_async16(to, kp + i * 512);
+          cp_async16(to + C::kCodes, vp + i * 512);
+        }
+        if (lane < 2 * halves) cp_async4(scale_dst + lane * 4, ((lane & 1) ? c.v_scales : c.k_scales) + ph);
+      };
+      auto issue = [&](int u, int2 ids, int stage) {
         if (u < last_code) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int pos = u * kUnit + 16 * e;
-            if (pos < code_end) {
-              const uint32_t dst = ring_a + stage * C::kStage + e * 2 * C::kHalf;
-              const uint32_t scale_dst = ring_a + stage * C::kStage + 4 * C::kHalf + e * 8;
-              const int id = ids[e];
-              if (id < 0 || id >= c.num_pages) {
-                if (lane == 0) atomicExch(error_word, LQ_BLOCK_BAD_PAGE);
-                if (lane < 2) asm volatile("st.shared.u32 [%0], %1;" ::"r"(scale_dst + lane * 4), "r"(0x7fffffff) : "memory");
-              } else {
-                const int64_t ph = (int64_t)id * c.kv_heads + h;
-                const int64_t at = ((ph << shift) + (pos & (P - 1))) * D + lane * 16;
-#pragma unroll
-                for (int i = 0; i < C::kHalf / 512; ++i) {
-                  const int idx = i * 32 + lane;
-                  const uint32_t piece = piece_at<D>(idx / (D / 16), idx % (D / 16));
-                  cp_async16(dst + piece, c.k_pages + at + i * 512);
-                  cp_async16(dst + C::kHalf + piece, c.v_pages + at + i * 512);
-                }
-                if (lane < 2) cp_async4(scale_dst + lane * 4, (lane ? c.v_scales : c.k_scales) + ph);
-              }
-            }
+          const int pos = u * kUnit;
+          if (P != 16) {
+            copy(ids.x, pos & (P - 1), 0, stage, std::integral_constant<int, 2>());
+          } else {
+            copy(ids.x, 0, 0, stage, std::integral_constant<int, 1>());
+            if (pos + 16 < code_end) copy(ids.y, 0, 1, stage, std::integral_constant<int, 1>());
           }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
-      look_up(ua + warp);
+      int2 page[C::kStages];
 #pragma unroll
-      for (int i = 0; i < C::kStages - 1; ++i) {
-        issue(ua + warp + i * W, i);
-        look_up(ua + warp + (i + 1) * W);
-      }
-
-      // ---- the tile's query rows as fp16, each lifted by a power of two
-      for (int r = warp; r < ROWS; r += W) {
-        const int row = rt * sh.tile + r, t = row / sh.G, g = row - t * sh.G;
-        const bool live = row < sh.rows && t < x.s.n;
-        float v[D / 32], amax = 0.f;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          v[i] = live ? Conv<T>::to_f32(q[b * qsb + t * qst + (int64_t)(h * sh.G + g) * qsh + lane + 32 * i]) : 0.f;
-          amax = fmaxf(amax, finite_abs(v[i]));
-        }
-        float unit;
-        const float lift = lift_of(warp_max(amax), 10, unit);
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) q_s[r * C::kQ + lane + 32 * i] = __float2half_rn(v[i] * lift);
-        if (lane == 0) unit_s[r] = unit * qk_scale;
-      }
-      __syncthreads();
-
-      // this thread's query rows are 8 nt + 2 q4 (+ 1): their units and last visible positions
-      float qu[NT][2];
-      int seen[NT][2];
-      uint32_t qb[NT][KS][2];
+      for (int i = 0; i < C::kStages; ++i) page[i] = look_up(ua + i);
+      // the query rows: row 8 nt + gid, dims from q4 * 16 J on (requested before the codes, which wait for
+      // their page ids)
+      uint32_t raw[NT][8 * J];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
+        const int row = rt * sh.tile + nt * 8 + gid, t = token_of(sh, row), g = row - t * sh.G;
+        load_words(raw[nt], reinterpret_cast<const uint16_t*>(q) + b * qsb + t * qst + (int64_t)(h * sh.G + g) * qsh + q4 * 16 * J,
+                   row < sh.rows && t < x.s.n, q_vec);
+      }
+      __syncwarp();  // every lane is done with the last segment's units
+#pragma unroll
+      for (int i = 0; i < C::kStages - 1; ++i) issue(ua + i, page[i], i);
+      int2 next_page = page[C::kStages - 1];
+
+      // ---- the query rows as B operands, each lifted by a power of two. k-step k is the four (kInt: eight)
+      // dims from q4 * 16 J + 4 k (8 k) on; kInt: two k-steps hold the high and the low bytes of one.
+      uint32_t qb[NT][KS][2];
+      float qu[NT][2];   // what 1 of a product stands for, of the query rows 8 nt + 2 q4 (+ 1)
+      float qlift[NT];   // of row 8 nt + gid
+      int seen[NT][2];   // last position those rows see
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float amax = 0.f;
+        bool finite = true;
+#pragma unroll
+        for (int i = 0; i < 8 * J; ++i) {
+          const float2 v = pair_of<T>(raw[nt][i]);
+          finite = finite && fabsf(v.x) <= 3.402823466e38f && fabsf(v.y) <= 3.402823466e38f;
+          amax = fmaxf(amax, fmaxf(finite_abs(v.x), finite_abs(v.y)));
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        float unit;
+        qlift[nt] = lift_of(amax, kTop, unit);
+        // (integers cannot carry a NaN: a row that is not finite gets it with its unit)
+        const unsigned bad = __ballot_sync(0xffffffffu, !finite);
+        unit = (bad >> (gid * 4)) & 15u ? __int_as_float(0x7fffffff) : unit * qk_scale;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int r = nt * 8 + q4 * 2 + e;
-          qu[nt][e] = unit_s[r];
-          seen[nt][e] = x.s.start + (rt * sh.tile + r) / sh.G;
+          qu[nt][e] = __shfl_sync(0xffffffffu, unit, (q4 * 2 + e) * 4);
+          seen[nt][e] = x.s.start + token_of(sh, rt * sh.tile + nt * 8 + q4 * 2 + e);
         }
+        if constexpr (kInt) {
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {  // k-step k: the four dims from q4 * 16 J + 4 k on
-          const uint2 v = *reinterpret_cast<const uint2*>(q_s + (nt * 8 + gid) * C::kQ + q4 * 16 * J + k * 4);
-          qb[nt][k][0] = v.x;
-          qb[nt][k][1] = v.y;
+          for (int k = 0; k < 2 * J; ++k) {
+            uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 v = pair_of<T>(raw[nt][4 * k + i]);
+              const int a0 = __float2int_rn(v.x * qlift[nt]), a1 = __float2int_rn(v.y * qlift[nt]);  // |a| < 2^14
+              hi[i >> 1] |= ((uint32_t)((a0 + 128) >> 8) & 255u) << (16 * (i & 1)) | ((uint32_t)((a1 + 128) >> 8) & 255u) << (16 * (i & 1) + 8);
+              lo[i >> 1] |= ((uint32_t)a0 & 255u) << (16 * (i & 1)) | ((uint32_t)a1 & 255u) << (16 * (i & 1) + 8);
+            }
+            qb[nt][2 * k][0] = hi[0]; qb[nt][2 * k][1] = hi[1];
+            qb[nt][2 * k + 1][0] = lo[0]; qb[nt][2 * k + 1][1] = lo[1];
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float2 v = pair_of<T>(raw[nt][2 * k + i]);
+              qb[nt][k][i] = as_u32(__floats2half2_rn(v.x * qlift[nt], v.y * qlift[nt]));
+            }
         }
       }
       float o[NT][MT][4], m[NT][2], l[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        m[nt][0] = m[nt][1] = -INFINITY;
+        m[nt][0] = m[nt][1] = kNone;
         l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
         for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
@@ -348,19 +419,17 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
       // operands of the value product
       auto weigh = [&](auto& acc, auto& wb, int pos0, int end, const auto& ks, const auto& vs) {
         constexpr int H = sizeof(ks) / sizeof(float);
-        const bool masked = pos0 + 16 * H - 1 > min(first_seen, end - 1);
-        bool rises = false;
         float inv[H];
 #pragma unroll
         for (int e = 0; e < H; ++e) {
-          const float lv = __log2f(vs[e]);
-          inv[e] = inverse_of(vs[e]);
+          const float lv = log2_of(vs[e]);
+          inv[e] = fminf(inverse_of(vs[e]), 3.0e38f);  // (of a NaN scale: a number; the weights are NaN then)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[e][nt][i] = fmaf(acc[e][nt][i], qu[nt][i & 1] * ks[e], lv);
         }
-        if (masked) {
+        if (pos0 + 16 * H - 1 > min(first_seen, end - 1)) {
 #pragma unroll
           for (int e = 0; e < H; ++e)
 #pragma unroll
@@ -371,12 +440,16 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
                 if (pos > seen[nt][i & 1] || pos >= end) acc[e][nt][i] = -INFINITY;
               }
         }
+        bool rises = false;
+        float mx[NT][2];
 #pragma unroll
-        for (int e = 0; e < H; ++e)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) rises = rises || fmaxf(acc[e][nt][i], acc[e][nt][i + 2]) > m[nt][i] + 8.f;
+          for (int i = 0; i < 2; ++i) {
+            mx[nt][i] = fmaxf(acc[0][nt][i], acc[0][nt][i + 2]);
+            if (H == 2) mx[nt][i] = fmaxf(mx[nt][i], fmaxf(acc[H - 1][nt][i], acc[H - 1][nt][i + 2]));
+            rises = rises || mx[nt][i] > m[nt][i] + 8.f;
+          }
         // M follows the maximum only when a weight would pass 2^8: any M serves, and fp16 keeps 11
         // bits of a weight up to 2^15
         if (__any_sync(0xffffffffu, rises)) {
@@ -384,13 +457,11 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              float mx = fmaxf(acc[0][nt][i], acc[0][nt][i + 2]);
-              if (H == 2) mx = fmaxf(mx, fmaxf(acc[H - 1][nt][i], acc[H - 1][nt][i + 2]));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              const float to = fmaxf(m[nt][i], mx);
-              const float corr = m[nt][i] == -INFINITY ? 0.f : exp2_of(m[nt][i] - to);
+              float to = fmaxf(mx[nt][i], __shfl_xor_sync(0xffffffffu, mx[nt][i], 4));
+              to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 8));
+              to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 16));
+              to = fmaxf(to, m[nt][i]);
+              const float corr = exp2_of(m[nt][i] - to);
               m[nt][i] = to;
               l[nt][i] *= corr;
 #pragma unroll
@@ -401,65 +472,88 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
             }
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const float base0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], base1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < H; ++e) {
             float w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = exp2_of(acc[e][nt][i] - ((i & 1) ? base1 : base0));
-            // the sum takes the weights as they are multiplied, rounded to fp16: their rounding then
-            // cancels where few weights dominate. (Below 2^-14, where fp16 loses bits, it takes them
-            // as they are: a block of small values has small w but counts in the sum by w / vs.)
-            const __half2 w0 = __floats2half2_rn(w[0], w[1]), w1 = __floats2half2_rn(w[2], w[3]);
-            const float2 f0 = __half22float2(w0), f1 = __half22float2(w1);
-            const float least = 6.103515625e-05f;
-            const float sum0 = (w[0] < least ? w[0] : f0.x) + (w[2] < least ? w[2] : f1.x);
-            const float sum1 = (w[1] < least ? w[1] : f0.y) + (w[3] < least ? w[3] : f1.y);
-            l[nt][0] += sum0 == 0.f ? 0.f : sum0 * inv[e];  // (a masked token's scale may be NaN)
-            l[nt][1] += sum1 == 0.f ? 0.f : sum1 * inv[e];
-            wb[e][nt][0] = transpose8x8(as_u32(w0));
-            wb[e][nt][1] = transpose8x8(as_u32(w1));
+            for (int i = 0; i < 4; ++i) w[i] = exp2_of(acc[e][nt][i] - m[nt][i & 1]);
+            // (the sum takes the weights in fp32: a block of small values has weights that fp16 would
+            // lose, but counts in the sum by w / vs)
+            l[nt][0] = fmaf(w[0] + w[2], inv[e], l[nt][0]);
+            l[nt][1] = fmaf(w[1] + w[3], inv[e], l[nt][1]);
+            wb[e][nt][0] = transpose8x8(as_u32(__floats2half2_rn(w[0], w[1])));
+            wb[e][nt][1] = transpose8x8(as_u32(__floats2half2_rn(w[2], w[3])));
           }
-        }
       };
 
       // ---- complete blocks
       int stage = 0;
 #pragma unroll 1
-      for (int u = ua + warp; u < last_code; u += W) {
+      for (int u = ua; u < last_code; ++u) {
         __syncwarp();  // every lane is done with the unit before
-        issue(u + (C::kStages - 1) * W, stage == 0 ? C::kStages - 1 : stage - 1);
-        look_up(u + C::kStages * W);
+        issue(u + C::kStages - 1, next_page, stage == 0 ? C::kStages - 1 : stage - 1);
+        next_page = look_up(u + C::kStages);
         asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
         __syncwarp();  // the unit is there for every lane
         const uint32_t at = ring_a + stage * C::kStage;
         stage = stage + 1 == C::kStages ? 0 : stage + 1;
-        const uint4 sc = lds128m(at + 4 * C::kHalf);
+        const uint4 sc = lds128m(at + 2 * C::kCodes);
         float acc[2][NT][4];
+        if constexpr (kInt) {
+          int sum[2][NT][2][4];
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+          for (int e = 0; e < 2; ++e)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) acc[e][nt][0] = acc[e][nt][1] = acc[e][nt][2] = acc[e][nt][3] = 0.f;
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-          uint4 kx[2], ky[2];
+              for (int i = 0; i < 4; ++i) sum[e][nt][0][i] = sum[e][nt][1][i] = 0;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            kx[e] = lds128m(at + e * 2 * C::kHalf + piece_at<D>(gid, q4 * J + j));
-            ky[e] = lds128m(at + e * 2 * C::kHalf + piece_at<D>(gid + 8, q4 * J + j));
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
+          for (int j = 0; j < J; ++j)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const uint32_t xw = (k == 0 ? kx[e].x : k == 1 ? kx[e].y : k == 2 ? kx[e].z : kx[e].w) ^ 0x80808080u;
-              const uint32_t yw = (k == 0 ? ky[e].x : k == 1 ? ky[e].y : k == 2 ? ky[e].z : ky[e].w) ^ 0x80808080u;
-              const uint32_t a0 = codes_h2(xw, 0x4140u), a1 = codes_h2(yw, 0x4140u);
-              const uint32_t a2 = codes_h2(xw, 0x4342u), a3 = codes_h2(yw, 0x4342u);
+              const uint4 kx = lds128m(at + k_at[j] + e * 16 * D), ky = lds128m(at + k_at[j] + e * 16 * D + 8 * D);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma16(acc[e][nt], a0, a1, a2, a3, qb[nt][4 * j + k][0], qb[nt][4 * j + k][1]);
+              for (int k = 0; k < 2; ++k) {
+                const uint32_t a0 = k ? kx.z : kx.x, a1 = k ? ky.z : ky.x, a2 = k ? kx.w : kx.y, a3 = k ? ky.w : ky.y;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int plane = 0; plane < 2; ++plane)
+                    mma8(sum[e][nt][plane], a0, a1, a2, a3, qb[nt][(2 * j + k) * 2 + plane][0], qb[nt][(2 * j + k) * 2 + plane][1]);
+              }
             }
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) acc[e][nt][i] = (float)(sum[e][nt][0][i] * 256 + sum[e][nt][1][i]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) acc[e][nt][0] = acc[e][nt][1] = acc[e][nt][2] = acc[e][nt][3] = 0.f;
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            uint4 kx[2], ky[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              kx[e] = lds128m(at + k_at[j] + e * 16 * D);
+              ky[e] = lds128m(at + k_at[j] + e * 16 * D + 8 * D);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t xw = (k == 0 ? kx[e].x : k == 1 ? kx[e].y : k == 2 ? kx[e].z : kx[e].w) ^ 0x80808080u;
+                const uint32_t yw = (k == 0 ? ky[e].x : k == 1 ? ky[e].y : k == 2 ? ky[e].z : ky[e].w) ^ 0x80808080u;
+                const uint32_t a0 = codes_h2(xw, 0x4140u), a1 = codes_h2(yw, 0x4140u);
+                const uint32_t a2 = codes_h2(xw, 0x4342u), a3 = codes_h2(yw, 0x4342u);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma16(acc[e][nt], a0, a1, a2, a3, qb[nt][4 * j + k][0], qb[nt][4 * j + k][1]);
+              }
+          }
         }
         const float ks[2] = {__uint_as_float(sc.x), __uint_as_float(sc.z)};
         const float vs[2] = {__uint_as_float(sc.y), __uint_as_float(sc.w)};
@@ -468,16 +562,15 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
         // row gid of value tile i is dim gid * DPT + 2 i, row gid + 8 the one after it
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint32_t v_a = at + (2 * e + 1) * C::kHalf;
           uint32_t vw[4][DPT / 4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {  // tokens 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9
-            const int row = q4 * 2 + (k & 1) + (k >> 1) * 8;
+            const uint32_t from = at + v_at[k & 1] + e * 16 * D + (k >> 1) * 8 * D;
             if (D == 128) {
-              const uint4 v = lds128m(v_a + piece_at<D>(row, gid));
+              const uint4 v = lds128m(from);
               vw[k][0] = v.x; vw[k][1] = v.y; vw[k][DPT / 4 - 2] = v.z; vw[k][DPT / 4 - 1] = v.w;
             } else {
-              const uint2 v = lds64(v_a + piece_at<D>(row, gid >> 1) + (gid & 1) * 8);
+              const uint2 v = lds64(from);
               vw[k][0] = v.x; vw[k][1] = v.y;
             }
           }
@@ -504,12 +597,10 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
 
       // ---- rows of the incomplete block, 16 at a time: lifted by a power of two of their own and taken
       // as fp16 (a bf16 value has 8 significant bits; what is lost lies 2^-24 below the largest)
-      const int first_tail = max(ua, x.code_units);
-      const int ahead = (warp + W - (first_tail - ua) % W) % W;  // units go round the warps without a break
 #pragma unroll 1
-      for (int i16 = 2 * (first_tail + ahead); i16 < 2 * ub; i16 += (i16 & 1) ? 2 * W - 1 : 1) {
+      for (int i16 = 2 * max(ua, x.code_units); i16 < 2 * ub; ++i16) {
         const int pos0 = x.held + (i16 - 2 * x.code_units) * 16;
-        if (pos0 >= x.visible) continue;
+        if (pos0 >= x.visible) break;
         const int L = x.s.start + x.s.n;
         const int64_t bh = ((int64_t)b * c.kv_heads + h) * 2 * P;
         float acc[1][NT][4];
@@ -548,7 +639,9 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
 #pragma unroll
           for (int i = 0; i < DPT / 8; ++i) largest(value_piece(e, i), vmax);
         float ks[1], vs[1];
-        const float klift = lift_of(warp_max(kmax), 10, ks[0]), vlift = lift_of(warp_max(vmax), 7, vs[0]);
+        const float klift = lift_of(warp_max(kmax), 10, ks[0]);
+        if (kInt) ks[0] *= 8.f;  // the fp16 queries are lifted 2^3 less than the integers
+        const float vlift = lift_of(warp_max(vmax), 7, vs[0]);
         auto lifted = [](uint32_t v, float lift) {
           const float2 p = pair_of<T>(v);
           return as_u32(__floats2half2_rn(p.x * lift, p.y * lift));
@@ -562,7 +655,17 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
             const uint32_t a0 = lifted(xs[2 * k], klift), a1 = lifted(ys[2 * k], klift);
             const uint32_t a2 = lifted(xs[2 * k + 1], klift), a3 = lifted(ys[2 * k + 1], klift);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16(acc[0][nt], a0, a1, a2, a3, qb[nt][2 * i + k][0], qb[nt][2 * i + k][1]);
+            for (int nt = 0; nt < NT; ++nt) {
+              uint32_t b0 = qb[nt][2 * i + k][0], b1 = qb[nt][2 * i + k][1];
+              if constexpr (kInt) {  // the integers put together again: 15 bits, of which fp16 takes 11; and exactly
+                // as many as a bf16 query had, down to 2^-14 of its row's largest
+                const uint32_t hi = qb[nt][2 * i][k], lo = qb[nt][2 * i + 1][k];
+                auto whole = [&](int n) { return (float)((int)(int8_t)(hi >> (8 * n)) * 256 + (int)(int8_t)(lo >> (8 * n))) * 0.125f; };
+                b0 = as_u32(__floats2half2_rn(whole(0), whole(1)));
+                b1 = as_u32(__floats2half2_rn(whole(2), whole(3)));
+              }
+              mma16(acc[0][nt], a0, a1, a2, a3, b0, b1);
+            }
           }
         }
         uint32_t wb[1][NT][2];
@@ -586,9 +689,9 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
         }
       }
 
-      // ---- merge the warps, each one's outputs in its drained ring
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-      __syncwarp();
+      // ---- what this run has of the (sequence, head): all of it, or a part
+      const bool whole = ua == 0 && ub == x.units;
+      const int64_t slot = ((int64_t)rt * (gridDim.x + heads) + blockIdx.x + b * c.kv_heads + h) * ROWS;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -597,125 +700,144 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
           sum += __shfl_xor_sync(0xffffffffu, sum, 4);
           sum += __shfl_xor_sync(0xffffffffu, sum, 8);
           sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-          const int r = nt * 8 + q4 * 2 + e;
-          if (gid == 0) ml_s[warp * ROWS + r] = make_float2(m[nt][e], sum);
-          float* dst = reinterpret_cast<float*>(ring) + r * C::kO + gid * DPT;
+          const int r = nt * 8 + q4 * 2 + e, row = rt * sh.tile + r, t = token_of(sh, row), g = row - t * sh.G;
+          if (row >= sh.rows) continue;
+          if (whole) {
+            // (1 / sum is exact enough: one rounding of 2^-24 before the one of T)
+            const float inv = t < x.s.n ? 1.f / sum : 0.f;
+            uint32_t w[MT];
 #pragma unroll
-          for (int i = 0; i < MT; ++i) *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[nt][i][e], o[nt][i][e + 2]);
+            for (int i = 0; i < MT; ++i)
+              w[i] = t < x.s.n ? pair_to<T>(o[nt][i][e] * inv, o[nt][i][e + 2] * inv) : 0u;
+            uint4* dst = reinterpret_cast<uint4*>(out + (((int64_t)b * sp.tokens + t) * sh.Hq + h * sh.G + g) * D + gid * DPT);
+#pragma unroll
+            for (int i = 0; i < MT / 4; ++i) dst[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          } else {
+            float4* dst = reinterpret_cast<float4*>(part + (slot + r) * D + gid * DPT);
+#pragma unroll
+            for (int i = 0; i < MT / 2; ++i)
+              dst[i] = make_float4(o[nt][2 * i][e], o[nt][2 * i][e + 2], o[nt][2 * i + 1][e], o[nt][2 * i + 1][e + 2]);
+            if (gid == 0) part_ml[slot + r] = make_float2(m[nt][e], sum);
+          }
         }
-      __syncthreads();
-      const bool whole = ua == 0 && ub == x.units;
-      const int64_t slot = ((int64_t)rt * (gridDim.x + heads) + cta + b * c.kv_heads + h) * ROWS;
-      const int some = min(W, ub - ua);  // warps that had units
-#pragma unroll 1
-      for (int i = threadIdx.x; i < ROWS * D / 4; i += C::kThreads) {
-        const int r = i / (D / 4), d = i % (D / 4) * 4;
-        const int row = rt * sh.tile + r, t = row / sh.G, g = row - t * sh.G;
-        if (row >= sh.rows) break;  // (rows rise with i)
-        float top = -INFINITY;
-        for (int w = 0; w < some; ++w) top = fmaxf(top, ml_s[w * ROWS + r].x);
-        float sum = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int w = 0; w < some; ++w) {
-          const float2 ml = ml_s[w * ROWS + r];
-          // (nothing visible: -inf and no sum; NaN scores: NaN sums, which must count)
-          const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_of(ml.x - top);
-          const float4 v = *reinterpret_cast<const float4*>(smem + (size_t)w * C::kWarpBytes + ((size_t)r * C::kO + d) * 4);
-          sum = fmaf(ml.y, f, sum);
-          acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y);
-          acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
-        }
-        if (whole) {
-          T* dst = out + (((int64_t)b * sp.tokens + t) * sh.Hq + h * sh.G + g) * D + d;
-          const bool live = t < x.s.n;
-          dst[0] = Conv<T>::from_f32(live ? acc.x / sum : 0.f);
-          dst[1] = Conv<T>::from_f32(live ? acc.y / sum : 0.f);
-          dst[2] = Conv<T>::from_f32(live ? acc.z / sum : 0.f);
-          dst[3] = Conv<T>::from_f32(live ? acc.w / sum : 0.f);
-        } else {
-          *reinterpret_cast<float4*>(part + (slot + r) * D + d) = acc;
-          if (d == 0) part_ml[slot + r] = make_float2(top, sum);
-        }
-      }
-      __syncthreads();  // the shared memory is free for the next (sequence, head)
     }
     off -= x.units * c.kv_heads;  // zero where the run goes on into the next sequence
   }
 }
 
 // ---------------------------------------------------------------- join the parts
-// grid (KV heads x rows of a tile, batch, row tiles), four warps: an output row that several CTAs
-// shared is the weighted sum of their parts; one that none took (it does not count) becomes
-// zeros. A warp takes every fourth part, a lane D / 32 of its values.
-constexpr int kJoinWarps = 4;
+// grid (sequences x KV heads, groups of `rows_each` rows of a tile, row tiles): an output row that
+// several warps shared is the weighted sum of their parts; one that none took (it does not count)
+// becomes zeros. A thread has four values of a row and every `groups`-th part.
+constexpr int kJoinMost = 1024;    // threads
+constexpr int kJoinBatch = 1024;   // weights held at a time: parts x rows
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinWarps * 32)
-block_attn_join_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, int ctas, T* __restrict__ out,
+__global__ void __launch_bounds__(kJoinMost)
+block_attn_join_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, int runs, int rows_each, T* __restrict__ out,
                        const float* __restrict__ part, const float2* __restrict__ part_ml, int* error_word) {
-  constexpr int V = D / 32;
-  __shared__ float acc_s[kJoinWarps][D], sum_s[kJoinWarps];
+  constexpr int V = D / 4;  // threads to a row
+  __shared__ float f_s[kJoinBatch], top_s[16];
+  __shared__ float4 acc_s[kJoinMost];
+  __shared__ int4 place_s;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int h = blockIdx.x % c.kv_heads, r = blockIdx.x / c.kv_heads, b = blockIdx.y, rt = blockIdx.z;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row = rt * sh.tile + r, t = row / sh.G, g = row - t * sh.G;
-  if (row >= sh.rows) return;
-  // (start and count are older than the kernel ahead, which has waited for their writer)
-  const Tile x = tile_of(c, sp, sh, b, rt);
   const int heads = c.batch * c.kv_heads;
-  int c0 = 0, c1 = -1;
-  if (x.units > 0) {
-    const int2 line = units_before(c, sp, sh, rt, b);
-    const Cut cut = cut_of(line.x, ctas, heads, sh.warps);
-    c0 = cut.owner(line.y + h * x.units);
-    c1 = cut.owner(line.y + (h + 1) * x.units - 1);
-  }
-  T* dst = out + (((int64_t)b * sp.tokens + t) * sh.Hq + h * sh.G + g) * D;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (x.units > 0 && c0 == c1) return;  // one CTA had all of it and wrote the output
-  if (x.bad && threadIdx.x == 0) atomicExch(error_word, LQ_BLOCK_BAD_POSITION);
-  if (x.units == 0 || t >= x.s.n) {
-    for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) dst[d] = Conv<T>::from_f32(0.f);
-    return;
-  }
-  const int64_t slot = ((int64_t)rt * (ctas + heads) + b * c.kv_heads + h + c0) * sh.tile + r;
-  const int parts = c1 - c0 + 1;
-  const float2* ml = part_ml + slot;
-  const float* mine = part + slot * D + lane * V;
-  float top = -INFINITY;
-  for (int k = lane; k < parts; k += 32) top = fmaxf(top, ml[(int64_t)k * sh.tile].x);
-  top = warp_max(top);
-  float sum = 0.f, acc[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) acc[i] = 0.f;
-#pragma unroll 4
-  for (int k = warp; k < parts; k += kJoinWarps) {
-    const float2 w = ml[(int64_t)k * sh.tile];
-    const float f = w.x == -INFINITY ? (w.y == 0.f ? 0.f : 1.f) : exp2_of(w.x - top);
-    const float* v = mine + (int64_t)k * sh.tile * D;
-    sum = fmaf(w.y, f, sum);
-#pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = fmaf(v[i], f, acc[i]);
-  }
-  if (lane == 0) sum_s[warp] = sum;
-#pragma unroll
-  for (int i = 0; i < V; ++i) acc_s[warp][lane * V + i] = acc[i];
-  __syncthreads();
-  for (int d = threadIdx.x; d < D; d += kJoinWarps * 32) {
-    float v = 0.f, all = 0.f;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-      v += acc_s[w][d];
-      all += sum_s[w];
+  const int b = blockIdx.x / c.kv_heads, h = blockIdx.x - b * c.kv_heads, rt = blockIdx.z;
+  // (start and count are older than the kernel ahead, which has waited for their writer)
+  if (threadIdx.x < 32) {
+    const Tile x = tile_of(c, sp, sh, b, rt);
+    int c0 = 0, c1 = -1;
+    if (x.units > 0) {
+      const int2 line = units_before(c, sp, sh, rt, b);
+      const Cut cut(line.x, sh);
+      c0 = cut.owner(sh, line.y + h * x.units);
+      c1 = x.units == 1 ? c0 : cut.owner(sh, line.y + (h + 1) * x.units - 1);
     }
-    dst[d] = Conv<T>::from_f32(v / all);
+    if (threadIdx.x == 0) {
+      place_s = make_int4(c0, c1 - c0 + 1, x.s.n, 0);
+      if (x.bad) atomicExch(error_word, LQ_BLOCK_BAD_POSITION);
+    }
   }
+  __syncthreads();
+  const int parts = place_s.y, n = place_s.z;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (parts == 1) return;  // one warp had all of it and wrote the output
+  const int r0 = blockIdx.y * rows_each, rows = min(rows_each, min(sh.tile, sh.rows - rt * sh.tile) - r0);
+  if (rows <= 0) return;
+  const int64_t slot = ((int64_t)rt * (runs + heads) + blockIdx.x + place_s.x) * sh.tile + r0;
+  const float2* ml = part_ml + slot;  // [parts][tile]
+  const float* mine = part + slot * D;
+  const int items = rows * V, groups = blockDim.x / items > 0 ? blockDim.x / items : 1;
+  const int group = threadIdx.x / items, item = threadIdx.x - group * items, r = item / V, d = (item - r * V) * 4;
+  const bool works = group < groups;
+  // the maximum of each row: of what a thread sees, then (one row) of its warp, then of all
+  if (threadIdx.x < 16) top_s[threadIdx.x] = kNone;
+  __syncthreads();
+  const int lanes = blockDim.x / rows, ri = threadIdx.x % rows;
+  float top = kNone;
+  if ((int)threadIdx.x < lanes * rows)
+    for (int k = threadIdx.x / rows; k < parts; k += lanes) top = fmaxf(top, ml[(int64_t)k * sh.tile + ri].x);
+  if (rows == 1) top = warp_max(top);
+  if (top > kNone && (rows > 1 || (threadIdx.x & 31) == 0)) {
+    // (floats of one sign are ordered as integers are, or the other way round; a maximum has no ties to break)
+    if (top >= 0.f) atomicMax(reinterpret_cast<int*>(&top_s[ri]), __float_as_int(top));
+    else atomicMin(reinterpret_cast<unsigned*>(&top_s[ri]), __float_as_uint(top));
+  }
+  __syncthreads();
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  const int batch = kJoinBatch / rows;
+  for (int k0 = 0; k0 < parts; k0 += batch) {
+    const int here = min(batch, parts - k0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < here * rows; i += blockDim.x) {
+      const int k = i / rows, of = i - k * rows;
+      f_s[i] = exp2_of(ml[(int64_t)(k0 + k) * sh.tile + of].x - top_s[of]);
+    }
+    __syncthreads();
+    if (works) {
+      for (int k = group; k < here; k += 8 * groups) {
+        float4 v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int at = k + u * groups;
+          v[u] = at < here ? __ldcg(reinterpret_cast<const float4*>(mine + ((int64_t)(k0 + at) * sh.tile + r) * D + d))
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int at = k + u * groups;
+          const float f = at < here ? f_s[at * rows + r] : 0.f;
+          acc.x = fmaf(v[u].x, f, acc.x); acc.y = fmaf(v[u].y, f, acc.y);
+          acc.z = fmaf(v[u].z, f, acc.z); acc.w = fmaf(v[u].w, f, acc.w);
+          if (d == 0 && at < here) sum = fmaf(ml[(int64_t)(k0 + at) * sh.tile + r].y, f, sum);
+        }
+      }
+    }
+  }
+  // the groups together, in order
+  acc_s[threadIdx.x] = acc;
+  __syncthreads();
+  if (works && d == 0) f_s[group * rows + r] = sum;  // (groups * rows <= threads / V < kJoinBatch)
+  __syncthreads();
+  if (threadIdx.x >= items) return;
+  float all = 0.f;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int g = 0; g < groups; ++g) {
+    const float4 v = acc_s[g * items + item];
+    acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+    all += f_s[g * rows + r];
+  }
+  const int row = rt * sh.tile + r0 + r, t = token_of(sh, row), gq = row - t * sh.G;
+  const bool live = parts > 0 && t < n;
+  const float inv = live ? 1.f / all : 0.f;
+  uint2* dst = reinterpret_cast<uint2*>(out + (((int64_t)b * sp.tokens + t) * sh.Hq + h * sh.G + gq) * D + d);
+  *dst = live ? make_uint2(pair_to<T>(acc.x * inv, acc.y * inv), pair_to<T>(acc.z * inv, acc.w * inv)) : make_uint2(0u, 0u);
 }
 
 // ---------------------------------------------------------------- host
 struct Plan {
   Shape sh;
-  int nt, tiles, ctas;
+  int nt, tiles, runs;
 };
 
 Plan plan_of(const lq_block_kv& c, int Hq, int T_new) {
@@ -723,17 +845,20 @@ Plan plan_of(const lq_block_kv& c, int Hq, int T_new) {
   p.sh.Hq = Hq;
   p.sh.G = Hq / c.kv_heads;
   p.sh.rows = T_new * p.sh.G;
+  p.sh.inv_G = (0x100000000ULL + p.sh.G - 1) / p.sh.G;
   p.nt = p.sh.rows <= 8 ? 1 : 2;
   p.sh.tile = 8 * p.nt;
-  p.sh.warps = p.nt == 1 ? Cfg<128, 1>::kWarps : Cfg<128, 2>::kWarps;
   p.tiles = (p.sh.rows + p.sh.tile - 1) / p.sh.tile;
-  p.ctas = sm_count() / p.tiles;
-  if (p.ctas < 1) p.ctas = 1;
+  const int at_once = sm_count() * (p.nt == 1 ? Cfg<128, 1>::kWarps : Cfg<128, 2>::kWarps);
+  p.sh.slots = at_once / p.tiles > 1 ? at_once / p.tiles : 2;
+  p.sh.step = (uint32_t)(0x100000000ULL / p.sh.slots);
+  p.sh.waves = p.tiles == 1 ? 2 : 1;
+  p.runs = p.sh.waves * p.sh.slots;
   return p;
 }
 
 int64_t slots_of(const lq_block_kv& c, const Plan& p) {
-  return (int64_t)p.tiles * (p.ctas + (int64_t)c.batch * c.kv_heads) * p.sh.tile;
+  return (int64_t)p.tiles * (p.runs + (int64_t)c.batch * c.kv_heads) * p.sh.tile;
 }
 int64_t scratch_bytes(const lq_block_kv& c, const Plan& p) { return slots_of(c, p) * (c.head_dim + 2) * 4; }
 
@@ -742,7 +867,8 @@ int check_attn(const lq_block_kv* c, int Hq, int T_new, const char* what) {
   LQ_REQUIRE(Hq > 0 && Hq % c->kv_heads == 0 && T_new > 0, LQ_ERR_ARG,
              "%s: %d query heads do not share %d KV heads evenly, or there are no rows", what, Hq, c->kv_heads);
   LQ_REQUIRE(c->dtype != LQ_F32, LQ_ERR_UNSUPPORTED, "%s: built for float16 and bfloat16 rows", what);
-  LQ_REQUIRE(c->kv_heads <= 65535 && (int64_t)T_new * (Hq / c->kv_heads) <= 65535LL * 8, LQ_ERR_ARG,
+  const int64_t group = Hq / c->kv_heads, rows = T_new * group;
+  LQ_REQUIRE(c->kv_heads <= 65535 && rows <= 65535LL * 8 && (rows + 64) * group < 0x100000000LL, LQ_ERR_ARG,
              "%s: too many rows for one call", what);
   LQ_REQUIRE((int64_t)c->batch * c->kv_heads * ((int64_t)c->max_blocks * c->block / kUnit + 2) < 0x7fffffffLL, LQ_ERR_ARG,
              "%s: batch, heads and positions together are too many for one call", what);
@@ -773,18 +899,23 @@ template <typename T, int D, int NT>
 int run(const lq_block_kv& c, const BlockSpan& sp, const Plan& p, const void* q, const int64_t* qs, void* out, void* scratch,
         float scaling, int pdl, cudaStream_t stream, int* error_word, const char* what) {
   auto kern = block_attn_kernel<T, D, NT>;
-  constexpr size_t smem = Cfg<D, NT>::kTotal;
+  constexpr size_t smem = Cfg<D, NT>::kRing;
   if (const int rc = ensure_smem_limit(reinterpret_cast<const void*>(kern), (int)smem, what)) return rc;
   const float qk_scale = scaling * 1.4426950408889634f;
+  const int q_vec = (((uintptr_t)q | (uintptr_t)(qs[0] * 2) | (uintptr_t)(qs[1] * 2) | (uintptr_t)(qs[2] * 2)) & 15) == 0;
   float* part = (float*)scratch;
   float2* part_ml = (float2*)(part + slots_of(c, p) * D);
-  if (const int rc = launch(kern, dim3((unsigned)p.ctas, (unsigned)p.tiles), Cfg<D, NT>::kThreads, smem, stream, pdl, what, c, sp, p.sh,
-                            (const T*)q, qs[0], qs[1], qs[2], (T*)out, part, part_ml, qk_scale, error_word))
+  if (const int rc = launch(kern, dim3((unsigned)p.runs, (unsigned)p.tiles), 32, smem, stream, pdl, what, c, sp, p.sh,
+                            (const T*)q, qs[0], qs[1], qs[2], q_vec, (T*)out, part, part_ml, qk_scale, error_word))
     return rc;
-  const unsigned rows = (unsigned)(p.sh.rows < p.sh.tile ? p.sh.rows : p.sh.tile);
-  return launch(block_attn_join_kernel<T, D>, dim3((unsigned)c.kv_heads * rows, (unsigned)c.batch, (unsigned)p.tiles),
-                kJoinWarps * 32, 0, stream, 1, what, c, sp, p.sh, p.ctas, (T*)out, (const float*)part, (const float2*)part_ml,
-                error_word);
+  // Few (sequence, head)s have many parts each: a CTA of 1024 threads for each of their rows. Many have
+  // few parts: one CTA of 128 for all rows of a tile.
+  const int64_t tops = (int64_t)c.batch * c.kv_heads * p.tiles;
+  const int rows = p.sh.rows < p.sh.tile ? p.sh.rows : p.sh.tile;
+  const bool few = tops * rows <= sm_count();
+  const int each = few ? 1 : rows, threads = few ? 1024 : rows * D / 4 > 128 ? rows * D / 4 : 128;
+  return launch(block_attn_join_kernel<T, D>, dim3((unsigned)(c.batch * c.kv_heads), (unsigned)(rows / each), (unsigned)p.tiles),
+                threads, 0, stream, 1, what, c, sp, p.sh, p.runs, each, (T*)out, (const float*)part, (const float2*)part_ml, error_word);
 }
 
 template <typename T>

@@ -651,6 +651,7 @@ int check_block_kv(const lq_block_kv* c, const char* what) {
              "%s: the block-scaled cache is built for head_dim 64 and 128, got %d", what, c->head_dim);
   LQ_REQUIRE(c->block == 16 || c->block == 32 || c->block == 64 || c->block == 128, LQ_ERR_UNSUPPORTED,
              "%s: a block is 16, 32, 64 or 128 tokens, got %d", what, c->block);
+  LQ_REQUIRE(c->num_pages <= 0x7fffffffLL / c->kv_heads, LQ_ERR_ARG, "%s: the pool has too many pages", what);
   LQ_REQUIRE((int64_t)c->max_blocks * c->block <= 0x7fff0000LL, LQ_ERR_ARG, "%s: the table spans too many positions", what);
   LQ_REQUIRE(c->dtype == LQ_F32 || c->dtype == LQ_F16 || c->dtype == LQ_BF16, LQ_ERR_DTYPE,
              "%s: the cache's dtype must be float32, float16 or bfloat16, got dtype id %d", what, c->dtype);
