@@ -133,30 +133,7 @@ struct Cut {
     if (kind == 1 || i >= 2 * sh.slots) return total;
     return first + (int)((uint64_t)(total - first) * ((uint64_t)sh.step * (i - sh.slots)) >> 32);
   }
-  __device__ __forceinline__ int owner(const Shape& sh, int unit) const {  // begin(owner) <= unit < begin(owner + 1)
-    if (kind == 0) return unit;
-    const bool later = unit >= first;
-    const int wave = later ? sh.slots : 0, last = later ? 2 * sh.slots - 1 : sh.slots - 1;
-    const float per = (float)sh.slots / (float)(later ? total - first : first);
-    int i = min(last, wave + (int)((float)(unit - (later ? first : 0)) * per));
-    while (begin(sh, i) > unit) --i;
-    while (i < last && begin(sh, i + 1) <= unit) ++i;
-    return i;
-  }
 };
-
-// All units of row tile rt and, of those, the ones before sequence `b`. One warp calls it.
-__device__ __forceinline__ int2 units_before(const lq_block_kv& c, const BlockSpan& sp, const Shape& sh, int rt, int b) {
-  int total = 0, before = 0;
-  for (int i = threadIdx.x & 31; i < c.batch; i += 32) {
-    const int u = tile_of(c, sp, sh, i, rt).units;
-    total += u;
-    if (i < b) before += u;
-  }
-  total = __reduce_add_sync(0xffffffffu, total);
-  before = __reduce_add_sync(0xffffffffu, before);
-  return make_int2(total * c.kv_heads, before * c.kv_heads);
-}
 
 // Where run `run` of the line lies: its length, its first sequence, and its begin behind that
 // sequence's. One warp calls it.
@@ -187,14 +164,14 @@ __device__ __forceinline__ int3 run_of(const lq_block_kv& c, const BlockSpan& sp
 }
 
 // NT: groups of 8 query rows of a pass. The outputs take NT * D / 4 registers of a thread, so an SM holds 12
-// warps with one group and 8 with two; their rings fill its shared memory.
+// warps with one group of 128 dims (16 of 64 dims) and 8 with two; their rings fill its shared memory.
 template <int D, int NT>
 struct Cfg {
-  static constexpr int kWarps = NT == 1 ? 12 : 8;        // on an SM
+  static constexpr int kWarps = NT == 1 ? (D == 64 ? 16 : 12) : 8;  // on an SM
   static constexpr int kRows = 8 * NT;
   static constexpr int kCodes = kUnit * D;               // bytes of a unit's keys, or values
   static constexpr int kStage = 2 * kCodes + 16;         // keys, values, (key, value) scales of the two halves
-  static constexpr int kStages = (NT == 1 ? 2 : 3) * (128 / D);  // units in a warp's ring
+  static constexpr int kStages = NT == 1 ? (D == 64 ? 3 : 2) : (D == 64 ? 6 : 3);  // units in a warp's ring
   static constexpr size_t kRing = kStages * kStage;
   static_assert(kStage % 16 == 0 && kWarps * (kRing + 1024) <= 228 * 1024, "");
 };
@@ -243,13 +220,24 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint16_t* p, 
   }
 }
 
+// Largest magnitude of 16-bit pairs, INF if one is not finite
+template <typename T, int N>
+__device__ __forceinline__ float largest_of(const uint32_t (&w)[N]) {
+  using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  T2 top = __habs2(*reinterpret_cast<const T2*>(&w[0]));
+#pragma unroll
+  for (int i = 1; i < N; ++i) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const T2*>(&w[i])));
+  const float lo = __low2float(top), hi = __high2float(top);
+  return lo <= 3.402823466e38f && hi <= 3.402823466e38f ? fmaxf(lo, hi) : INFINITY;
+}
+
 // ---------------------------------------------------------------- main kernel
 // grid (runs of the line, row tiles), one warp. T is the type of q, out and the ring.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32, (Cfg<D, NT>::kWarps))
 block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const T* __restrict__ q, int64_t qsb, int64_t qst,
                   int64_t qsh, int q_vec, T* __restrict__ out, float* __restrict__ part, float2* __restrict__ part_ml,
-                  float qk_scale, int* error_word) {
+                  int2* __restrict__ ends, float qk_scale, int* error_word) {
   using C = Cfg<D, NT>;
   constexpr int ROWS = C::kRows, KS = D / 16, MT = D / 16, DPT = D / 8;  // DPT: dims of V a thread owns
   constexpr int J = D / 64;  // 16-byte pieces of a K row a thread reads
@@ -358,25 +346,16 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
       // dims from q4 * 16 J + 4 k (8 k) on; kInt: two k-steps hold the high and the low bytes of one.
       uint32_t qb[NT][KS][2];
       float qu[NT][2];   // what 1 of a product stands for, of the query rows 8 nt + 2 q4 (+ 1)
-      float qlift[NT];   // of row 8 nt + gid
       int seen[NT][2];   // last position those rows see
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float amax = 0.f;
-        bool finite = true;
-#pragma unroll
-        for (int i = 0; i < 8 * J; ++i) {
-          const float2 v = pair_of<T>(raw[nt][i]);
-          finite = finite && fabsf(v.x) <= 3.402823466e38f && fabsf(v.y) <= 3.402823466e38f;
-          amax = fmaxf(amax, fmaxf(finite_abs(v.x), finite_abs(v.y)));
-        }
+        float amax = largest_of<T>(raw[nt]);  // INF if a value is not finite
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         float unit;
-        qlift[nt] = lift_of(amax, kTop, unit);
+        const float lift = lift_of(finite_abs(amax), kTop, unit);
         // (integers cannot carry a NaN: a row that is not finite gets it with its unit)
-        const unsigned bad = __ballot_sync(0xffffffffu, !finite);
-        unit = (bad >> (gid * 4)) & 15u ? __int_as_float(0x7fffffff) : unit * qk_scale;
+        unit = amax <= 3.402823466e38f ? unit * qk_scale : __int_as_float(0x7fffffff);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           qu[nt][e] = __shfl_sync(0xffffffffu, unit, (q4 * 2 + e) * 4);
@@ -384,25 +363,25 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
         }
         if constexpr (kInt) {
 #pragma unroll
-          for (int k = 0; k < 2 * J; ++k) {
-            uint32_t hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
+          for (int k = 0; k < 2 * J; ++k)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 v = pair_of<T>(raw[nt][4 * k + i]);
-              const int a0 = __float2int_rn(v.x * qlift[nt]), a1 = __float2int_rn(v.y * qlift[nt]);  // |a| < 2^14
-              hi[i >> 1] |= ((uint32_t)((a0 + 128) >> 8) & 255u) << (16 * (i & 1)) | ((uint32_t)((a1 + 128) >> 8) & 255u) << (16 * (i & 1) + 8);
-              lo[i >> 1] |= ((uint32_t)a0 & 255u) << (16 * (i & 1)) | ((uint32_t)a1 & 255u) << (16 * (i & 1) + 8);
+            for (int i = 0; i < 2; ++i) {
+              // whole + 128 in the low bits of a sum with 1.5 * 2^23, |whole| < 2^14: its second byte is the
+              // high byte (whole + 128) >> 8, its first the low byte plus 128
+              const float2 v0 = pair_of<T>(raw[nt][4 * k + 2 * i]), v1 = pair_of<T>(raw[nt][4 * k + 2 * i + 1]);
+              const uint32_t a0 = __float_as_uint(fmaf(v0.x, lift, 12583040.f)), a1 = __float_as_uint(fmaf(v0.y, lift, 12583040.f));
+              const uint32_t a2 = __float_as_uint(fmaf(v1.x, lift, 12583040.f)), a3 = __float_as_uint(fmaf(v1.y, lift, 12583040.f));
+              const uint32_t x01 = __byte_perm(a0, a1, 0x5140u), x23 = __byte_perm(a2, a3, 0x5140u);  // low, low, high, high
+              qb[nt][2 * k][i] = __byte_perm(x01, x23, 0x7632u);
+              qb[nt][2 * k + 1][i] = __byte_perm(x01, x23, 0x5410u) ^ 0x80808080u;
             }
-            qb[nt][2 * k][0] = hi[0]; qb[nt][2 * k][1] = hi[1];
-            qb[nt][2 * k + 1][0] = lo[0]; qb[nt][2 * k + 1][1] = lo[1];
-          }
         } else {
 #pragma unroll
           for (int k = 0; k < KS; ++k)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const float2 v = pair_of<T>(raw[nt][2 * k + i]);
-              qb[nt][k][i] = as_u32(__floats2half2_rn(v.x * qlift[nt], v.y * qlift[nt]));
+              qb[nt][k][i] = as_u32(__floats2half2_rn(v.x * lift, v.y * lift));
             }
         }
       }
@@ -692,6 +671,10 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
       // ---- what this run has of the (sequence, head): all of it, or a part
       const bool whole = ua == 0 && ub == x.units;
       const int64_t slot = ((int64_t)rt * (gridDim.x + heads) + blockIdx.x + b * c.kv_heads + h) * ROWS;
+      if (lane == 0) {  // for the join: the runs that begin and end it
+        if (ua == 0) ends[(int64_t)rt * heads + b * c.kv_heads + h].x = blockIdx.x;
+        if (ub == x.units) ends[(int64_t)rt * heads + b * c.kv_heads + h].y = blockIdx.x;
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -726,111 +709,93 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
 }
 
 // ---------------------------------------------------------------- join the parts
-// grid (sequences x KV heads, groups of `rows_each` rows of a tile, row tiles): an output row that
+// grid (sequences x KV heads, row groups x column groups of a tile, row tiles): an output row that
 // several warps shared is the weighted sum of their parts; one that none took (it does not count)
-// becomes zeros. A thread has four values of a row and every `groups`-th part.
-constexpr int kJoinMost = 1024;    // threads
-constexpr int kJoinBatch = 1024;   // weights held at a time: parts x rows
+// becomes zeros. A thread has four values of a row and every `groups`-th part, eight of them requested
+// at a time together with their (M, sum): three dependent trips to memory in all.
+constexpr int kJoinMost = 1024;  // threads
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinMost)
-block_attn_join_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, int runs, int rows_each, T* __restrict__ out,
-                       const float* __restrict__ part, const float2* __restrict__ part_ml, int* error_word) {
-  constexpr int V = D / 4;  // threads to a row
-  __shared__ float f_s[kJoinBatch], top_s[16];
+block_attn_join_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, int runs, int rows_each, int cols, T* __restrict__ out,
+                       const float* __restrict__ part, const float2* __restrict__ part_ml, const int2* __restrict__ ends,
+                       int* error_word) {
+  const int V = D / 4 / cols;  // threads to a row's share of columns
   __shared__ float4 acc_s[kJoinMost];
-  __shared__ int4 place_s;
+  __shared__ float2 ml_s[kJoinMost];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int heads = c.batch * c.kv_heads;
   const int b = blockIdx.x / c.kv_heads, h = blockIdx.x - b * c.kv_heads, rt = blockIdx.z;
   // (start and count are older than the kernel ahead, which has waited for their writer)
-  if (threadIdx.x < 32) {
-    const Tile x = tile_of(c, sp, sh, b, rt);
-    int c0 = 0, c1 = -1;
-    if (x.units > 0) {
-      const int2 line = units_before(c, sp, sh, rt, b);
-      const Cut cut(line.x, sh);
-      c0 = cut.owner(sh, line.y + h * x.units);
-      c1 = x.units == 1 ? c0 : cut.owner(sh, line.y + (h + 1) * x.units - 1);
-    }
-    if (threadIdx.x == 0) {
-      place_s = make_int4(c0, c1 - c0 + 1, x.s.n, 0);
-      if (x.bad) atomicExch(error_word, LQ_BLOCK_BAD_POSITION);
-    }
-  }
-  __syncthreads();
-  const int parts = place_s.y, n = place_s.z;
+  const Tile x = tile_of(c, sp, sh, b, rt);
+  const int r0 = blockIdx.y / cols * rows_each, rows = min(rows_each, min(sh.tile, sh.rows - rt * sh.tile) - r0);
+  const int items = rows * V, groups = max(1, (int)blockDim.x / items);
+  const int group = threadIdx.x / items, item = threadIdx.x - group * items, r = item / V, d = (item - r * V + blockIdx.y % cols * V) * 4;
+  const int row = rt * sh.tile + r0 + r, t = token_of(sh, row), g = row - t * sh.G;
+  uint2* dst = reinterpret_cast<uint2*>(out + (((int64_t)b * sp.tokens + t) * sh.Hq + h * sh.G + g) * D + d);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (parts == 1) return;  // one warp had all of it and wrote the output
-  const int r0 = blockIdx.y * rows_each, rows = min(rows_each, min(sh.tile, sh.rows - rt * sh.tile) - r0);
-  if (rows <= 0) return;
-  const int64_t slot = ((int64_t)rt * (runs + heads) + blockIdx.x + place_s.x) * sh.tile + r0;
-  const float2* ml = part_ml + slot;  // [parts][tile]
-  const float* mine = part + slot * D;
-  const int items = rows * V, groups = blockDim.x / items > 0 ? blockDim.x / items : 1;
-  const int group = threadIdx.x / items, item = threadIdx.x - group * items, r = item / V, d = (item - r * V) * 4;
-  const bool works = group < groups;
-  // the maximum of each row: of what a thread sees, then (one row) of its warp, then of all
-  if (threadIdx.x < 16) top_s[threadIdx.x] = kNone;
-  __syncthreads();
-  const int lanes = blockDim.x / rows, ri = threadIdx.x % rows;
-  float top = kNone;
-  if ((int)threadIdx.x < lanes * rows)
-    for (int k = threadIdx.x / rows; k < parts; k += lanes) top = fmaxf(top, ml[(int64_t)k * sh.tile + ri].x);
-  if (rows == 1) top = warp_max(top);
-  if (top > kNone && (rows > 1 || (threadIdx.x & 31) == 0)) {
-    // (floats of one sign are ordered as integers are, or the other way round; a maximum has no ties to break)
-    if (top >= 0.f) atomicMax(reinterpret_cast<int*>(&top_s[ri]), __float_as_int(top));
-    else atomicMin(reinterpret_cast<unsigned*>(&top_s[ri]), __float_as_uint(top));
+  if (x.bad && threadIdx.x == 0) atomicExch(error_word, LQ_BLOCK_BAD_POSITION);
+  if (x.units == 0) {
+    if (group == 0 && rows > 0) *dst = make_uint2(0u, 0u);
+    return;
   }
-  __syncthreads();
+  const int2 end = __ldcg(ends + (int64_t)rt * heads + blockIdx.x);
+  const int parts = end.y - end.x + 1;
+  if (parts == 1 || rows <= 0) return;  // one warp had all of it and wrote the output
+  const int64_t slot = ((int64_t)rt * (runs + heads) + blockIdx.x + end.x) * sh.tile + r0 + r;
+  const float2* ml = part_ml + slot;
+  const float* mine = part + slot * D + d;
+  float m = kNone, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
-  const int batch = kJoinBatch / rows;
-  for (int k0 = 0; k0 < parts; k0 += batch) {
-    const int here = min(batch, parts - k0);
-    __syncthreads();
-    for (int i = threadIdx.x; i < here * rows; i += blockDim.x) {
-      const int k = i / rows, of = i - k * rows;
-      f_s[i] = exp2_of(ml[(int64_t)(k0 + k) * sh.tile + of].x - top_s[of]);
-    }
-    __syncthreads();
-    if (works) {
-      for (int k = group; k < here; k += 8 * groups) {
-        float4 v[8];
+  if (group < groups) {
+    for (int k = group; k < parts; k += 8 * groups) {
+      float2 w[8];
+      float4 v[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int at = k + u * groups;
-          v[u] = at < here ? __ldcg(reinterpret_cast<const float4*>(mine + ((int64_t)(k0 + at) * sh.tile + r) * D + d))
-                           : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+      for (int u = 0; u < 8; ++u) {
+        const int at = k + u * groups;
+        w[u] = at < parts ? __ldcg(ml + (int64_t)at * sh.tile) : make_float2(kNone, 0.f);
+        v[u] = at < parts ? __ldcg(reinterpret_cast<const float4*>(mine + (int64_t)at * sh.tile * D)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float top = m;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int at = k + u * groups;
-          const float f = at < here ? f_s[at * rows + r] : 0.f;
-          acc.x = fmaf(v[u].x, f, acc.x); acc.y = fmaf(v[u].y, f, acc.y);
-          acc.z = fmaf(v[u].z, f, acc.z); acc.w = fmaf(v[u].w, f, acc.w);
-          if (d == 0 && at < here) sum = fmaf(ml[(int64_t)(k0 + at) * sh.tile + r].y, f, sum);
-        }
+      for (int u = 0; u < 8; ++u) top = fmaxf(top, w[u].x);
+      const float corr = exp2_of(m - top);
+      m = top;
+      l *= corr;
+      acc.x *= corr; acc.y *= corr; acc.z *= corr; acc.w *= corr;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float f = exp2_of(w[u].x - top);
+        l = fmaf(w[u].y, f, l);
+        acc.x = fmaf(v[u].x, f, acc.x); acc.y = fmaf(v[u].y, f, acc.y);
+        acc.z = fmaf(v[u].z, f, acc.z); acc.w = fmaf(v[u].w, f, acc.w);
       }
     }
   }
-  // the groups together, in order
-  acc_s[threadIdx.x] = acc;
-  __syncthreads();
-  if (works && d == 0) f_s[group * rows + r] = sum;  // (groups * rows <= threads / V < kJoinBatch)
-  __syncthreads();
-  if (threadIdx.x >= items) return;
-  float all = 0.f;
-  acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int g = 0; g < groups; ++g) {
-    const float4 v = acc_s[g * items + item];
-    acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
-    all += f_s[g * rows + r];
+  if (groups > 1) {
+    acc_s[threadIdx.x] = acc;
+    ml_s[threadIdx.x] = make_float2(m, l);
+    __syncthreads();
+    if (group == 0) {
+      float top = m;
+      const int used = min(groups, parts);
+      for (int k = 1; k < used; ++k) top = fmaxf(top, ml_s[k * items + item].x);
+      acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      l = 0.f;
+#pragma unroll 4
+      for (int k = 0; k < used; ++k) {
+        const float2 w = ml_s[k * items + item];
+        const float4 v = acc_s[k * items + item];
+        const float f = exp2_of(w.x - top);
+        l = fmaf(w.y, f, l);
+        acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y);
+        acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
+      }
+    }
   }
-  const int row = rt * sh.tile + r0 + r, t = token_of(sh, row), gq = row - t * sh.G;
-  const bool live = parts > 0 && t < n;
-  const float inv = live ? 1.f / all : 0.f;
-  uint2* dst = reinterpret_cast<uint2*>(out + (((int64_t)b * sp.tokens + t) * sh.Hq + h * sh.G + gq) * D + d);
+  if (group != 0) return;
+  const bool live = t < x.s.n;
+  const float inv = 1.f / l;
   *dst = live ? make_uint2(pair_to<T>(acc.x * inv, acc.y * inv), pair_to<T>(acc.z * inv, acc.w * inv)) : make_uint2(0u, 0u);
 }
 
@@ -849,7 +814,7 @@ Plan plan_of(const lq_block_kv& c, int Hq, int T_new) {
   p.nt = p.sh.rows <= 8 ? 1 : 2;
   p.sh.tile = 8 * p.nt;
   p.tiles = (p.sh.rows + p.sh.tile - 1) / p.sh.tile;
-  const int at_once = sm_count() * (p.nt == 1 ? Cfg<128, 1>::kWarps : Cfg<128, 2>::kWarps);
+  const int at_once = sm_count() * (p.nt == 2 ? Cfg<128, 2>::kWarps : c.head_dim == 64 ? Cfg<64, 1>::kWarps : Cfg<128, 1>::kWarps);
   p.sh.slots = at_once / p.tiles > 1 ? at_once / p.tiles : 2;
   p.sh.step = (uint32_t)(0x100000000ULL / p.sh.slots);
   p.sh.waves = p.tiles == 1 ? 2 : 1;
@@ -860,7 +825,9 @@ Plan plan_of(const lq_block_kv& c, int Hq, int T_new) {
 int64_t slots_of(const lq_block_kv& c, const Plan& p) {
   return (int64_t)p.tiles * (p.runs + (int64_t)c.batch * c.kv_heads) * p.sh.tile;
 }
-int64_t scratch_bytes(const lq_block_kv& c, const Plan& p) { return slots_of(c, p) * (c.head_dim + 2) * 4; }
+int64_t scratch_bytes(const lq_block_kv& c, const Plan& p) {
+  return slots_of(c, p) * (c.head_dim + 2) * 4 + (int64_t)p.tiles * c.batch * c.kv_heads * (int64_t)sizeof(int2);
+}
 
 int check_attn(const lq_block_kv* c, int Hq, int T_new, const char* what) {
   if (const int rc = check_block_kv(c, what)) return rc;
@@ -905,17 +872,21 @@ int run(const lq_block_kv& c, const BlockSpan& sp, const Plan& p, const void* q,
   const int q_vec = (((uintptr_t)q | (uintptr_t)(qs[0] * 2) | (uintptr_t)(qs[1] * 2) | (uintptr_t)(qs[2] * 2)) & 15) == 0;
   float* part = (float*)scratch;
   float2* part_ml = (float2*)(part + slots_of(c, p) * D);
+  int2* ends = (int2*)(part_ml + slots_of(c, p));
   if (const int rc = launch(kern, dim3((unsigned)p.runs, (unsigned)p.tiles), 32, smem, stream, pdl, what, c, sp, p.sh,
-                            (const T*)q, qs[0], qs[1], qs[2], q_vec, (T*)out, part, part_ml, qk_scale, error_word))
+                            (const T*)q, qs[0], qs[1], qs[2], q_vec, (T*)out, part, part_ml, ends, qk_scale,
+                            error_word))
     return rc;
-  // Few (sequence, head)s have many parts each: a CTA of 1024 threads for each of their rows. Many have
-  // few parts: one CTA of 128 for all rows of a tile.
+  // Few (sequence, head)s have many parts each (hundreds, one long context): a CTA of 512 threads for each
+  // quarter of a row, so that 64 and more parts are on their way together. Many have few parts: one CTA
+  // for all rows of a tile, in two groups.
   const int64_t tops = (int64_t)c.batch * c.kv_heads * p.tiles;
   const int rows = p.sh.rows < p.sh.tile ? p.sh.rows : p.sh.tile;
-  const bool few = tops * rows <= sm_count();
-  const int each = few ? 1 : rows, threads = few ? 1024 : rows * D / 4 > 128 ? rows * D / 4 : 128;
-  return launch(block_attn_join_kernel<T, D>, dim3((unsigned)(c.batch * c.kv_heads), (unsigned)(rows / each), (unsigned)p.tiles),
-                threads, 0, stream, 1, what, c, sp, p.sh, p.runs, each, (T*)out, (const float*)part, (const float2*)part_ml, error_word);
+  const bool few = tops * rows <= 2 * sm_count();
+  const int each = few ? 1 : rows, cols = few ? 4 : 1, threads = few ? 512 : 2 * rows * D / 4;
+  return launch(block_attn_join_kernel<T, D>, dim3((unsigned)(c.batch * c.kv_heads), (unsigned)(rows / each * cols), (unsigned)p.tiles),
+                threads, 0, stream, 1, what, c, sp, p.sh, p.runs, each, cols, (T*)out, (const float*)part, (const float2*)part_ml,
+                (const int2*)ends, error_word);
 }
 
 template <typename T>

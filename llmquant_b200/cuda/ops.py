@@ -93,5 +93,5 @@ def qk_norm_rope(q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=1e
                     k_out.data_ptr(), strides[2], strides[3], native.DTYPE_ID[q.dtype], batch, tokens, heads,
                     k.shape[2], dim, native.ptr(q_weight), native.ptr(k_weight), eps, cos.data_ptr(), sin.data_ptr(),
                     cos.shape[0], rot, int(interleaved), positions.data_ptr(), positions.stride(0),
-                    positions.stride(1), 0, native.stream_ptr(q.device))
+                    positions.stride(1), 1, native.stream_ptr(q.device))
     return q_out, k_out

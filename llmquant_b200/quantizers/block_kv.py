@@ -124,7 +124,7 @@ class BlockKVStore:
         if tuple(t.shape) != shape:
             raise RuntimeError(f"{name} must be {shape}, got {tuple(t.shape)}")
 
-    def append(self, k, v, start, count=None, pdl=False):
+    def append(self, k, v, start, count=None, pdl=True):
         """Store new rows k, v [batch, kv_heads, tokens, head_dim] (any strides, head_dim contiguous)."""
         if k.dim() != 4:
             raise RuntimeError(f"k must be [batch, kv_heads, tokens, head_dim], got {tuple(k.shape)}")
@@ -141,7 +141,7 @@ class BlockKVStore:
                    (ctypes.c_int64 * 3)(*v.stride()[:3]), tokens, *span, int(pdl))
 
     def append_qkv(self, qkv, cos, sin, start, count=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False,
-                   q_out=None, pdl=False):
+                   q_out=None, pdl=True):
         """From the fused projection's rows qkv [batch, tokens, q heads + 2 kv heads, head_dim]: queries and
         keys normed (weights given) and turned by their positions' angles, keys and values stored,
         queries returned as [batch, tokens, q heads, head_dim]. One launch; the same values as
@@ -182,7 +182,7 @@ class BlockKVStore:
             self._scratch_bytes[key] = need
         return need
 
-    def attend(self, q, start, count=None, scaling=None, out=None, scratch=None, pdl=False):
+    def attend(self, q, start, count=None, scaling=None, out=None, scratch=None, pdl=True):
         """Attention of the newest rows q [batch, tokens, q heads, head_dim] (head_dim contiguous) over the
         cache after their `append`: row t sees positions 0 .. start + t. Returns [batch, tokens,
         q heads, head_dim], zeros for rows behind `count`. float16 and bfloat16 caches. `scratch`
@@ -231,7 +231,7 @@ class BlockKVStore:
         k = torch.empty(shape, dtype=self.dtype, device=self.device)
         v = torch.empty(shape, dtype=self.dtype, device=self.device)
         if length:
-            self._call("lq_block_kv_read", k.data_ptr(), v.data_ptr(), length, *span, tokens, 0)
+            self._call("lq_block_kv_read", k.data_ptr(), v.data_ptr(), length, *span, tokens, 1)
         return k, v
 
     def check_device_errors(self):
