@@ -1,5 +1,3 @@
-import ctypes
-
 import torch
 import torch.nn.functional as F
 
@@ -31,22 +29,27 @@ def fake_quantize_cuda(x: torch.Tensor, args, return_scale: bool = False):
 
 def check_rope_tables(cos, sin, device, head_dim):
     """The rotated width of fp32 angle tables [table_len, rot / 2] on `device`."""
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+    shape = cos.shape
+    if len(shape) != 2 or shape != sin.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
         raise RuntimeError("cos and sin must be float32 tables of one shape [positions, rotated / 2]")
     if cos.device != device or sin.device != device or not (cos.is_contiguous() and sin.is_contiguous()):
         raise RuntimeError(f"cos and sin must be contiguous on {device}")
-    rot = 2 * cos.shape[1]
-    if rot == 0 or rot > head_dim or rot % 16:
+    rot = 2 * shape[1]
+    if rot == 0 or rot > head_dim or rot % 16 or shape[0] == 0:
         raise RuntimeError(f"the tables turn {rot} values: a multiple of 16 up to head_dim {head_dim} is needed")
-    return rot
+    return shape[0], rot
 
 
 def check_norm_weights(q_weight, k_weight, dtype, device, head_dim):
-    if (q_weight is None) != (k_weight is None):
+    """Their addresses (0: no norms)."""
+    if q_weight is None and k_weight is None:
+        return 0, 0
+    if q_weight is None or k_weight is None:
         raise RuntimeError("norm weights are given for both queries and keys or for neither")
     for w in (q_weight, k_weight):
-        if w is not None and (w.dtype != dtype or w.device != device or w.shape != (head_dim,) or not w.is_contiguous()):
+        if w.dtype is not dtype or w.device != device or w.shape != (head_dim,) or not w.is_contiguous():
             raise RuntimeError(f"a norm weight must be a contiguous {dtype} [{head_dim}] on {device}")
+    return q_weight.data_ptr(), k_weight.data_ptr()
 
 
 def qk_norm_rope(q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, out=None):
@@ -55,43 +58,45 @@ def qk_norm_rope(q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=1e
     q [B, T, Hq, D] and k [B, T, Hk, D] (any strides with D contiguous, e.g. slices of the fused
     projection's output; float32, float16 or bfloat16), cos / sin float32 [positions, rot / 2],
     positions int64 [B, T] (or expandable to it). Returns new (q, k), or writes `out` = (q, k),
-    which may be the inputs themselves. Weights [D] of q's dtype, both None for a model without
-    these norms. fp32 inside, one rounding. No gradient."""
-    if not (q.is_cuda and k.is_cuda):
-        raise RuntimeError("q and k must be CUDA tensors")
-    if q.dtype not in native.DTYPE_ID:
-        raise RuntimeError(f"q must be float32, float16 or bfloat16, got {q.dtype}")
-    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
-        raise RuntimeError(f"q and k must be [batch, tokens, heads, head_dim], got {tuple(q.shape)} and {tuple(k.shape)}")
-    if k.dtype != q.dtype or k.device != q.device:
-        raise RuntimeError("q and k must share dtype and device")
-    batch, tokens, heads, dim = q.shape
+    which may be the inputs themselves (but not overlap them otherwise). Weights [D] of q's dtype,
+    both None for a model without these norms. fp32 inside, one rounding. A position outside the
+    tables gives NaN. No gradient."""
+    device, dtype, shape, k_shape = q.device, q.dtype, q.shape, k.shape
+    if device.type != "cuda" or k.device != device:
+        raise RuntimeError("q and k must be CUDA tensors of one device")
+    if dtype not in native.DTYPE_ID:
+        raise RuntimeError(f"q must be float32, float16 or bfloat16, got {dtype}")
+    if k.dtype is not dtype:
+        raise RuntimeError(f"q and k must share a dtype, got {dtype} and {k.dtype}")
+    if len(shape) != 4 or len(k_shape) != 4 or shape[:2] != k_shape[:2] or shape[3] != k_shape[3]:
+        raise RuntimeError(f"q and k must be [batch, tokens, heads, head_dim], got {tuple(shape)} and {tuple(k_shape)}")
+    batch, tokens, heads, dim = shape
     if dim % 8 or not 16 <= dim <= 256:
         raise RuntimeError(f"head_dim must be a multiple of 8 in [16, 256], got {dim}")
-    rot = check_rope_tables(cos, sin, q.device, dim)
-    check_norm_weights(q_weight, k_weight, q.dtype, q.device, dim)
-    if positions.dtype != torch.int64 or positions.device != q.device:
-        raise RuntimeError(f"positions must be int64 on {q.device}")
-    positions = positions.expand(batch, tokens)
-    if q.stride(3) != 1:
+    table_len, rot = check_rope_tables(cos, sin, device, dim)
+    wq, wk = check_norm_weights(q_weight, k_weight, dtype, device, dim)
+    if positions.dtype is not torch.int64 or positions.device != device:
+        raise RuntimeError(f"positions must be int64 on {device}")
+    if positions.shape != shape[:2]:
+        positions = positions.expand(batch, tokens)
+    qs, ks = q.stride(), k.stride()
+    if qs[3] != 1:
         q = q.contiguous()
-    if k.stride(3) != 1:
+        qs = q.stride()
+    if ks[3] != 1:
         k = k.contiguous()
+        ks = k.stride()
     if out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        k_out = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+        q_out, k_out = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k))
     else:
         q_out, k_out = out
-        for t, like in ((q_out, q), (k_out, k)):
-            if t.shape != like.shape or t.dtype != q.dtype or t.device != q.device or t.stride(3) != 1:
+        for t, like in ((q_out, shape), (k_out, k_shape)):
+            if t.shape != like or t.dtype is not dtype or t.device != device or t.stride(3) != 1:
                 raise RuntimeError("out must hold tensors of the inputs' shape, dtype and device, head_dim contiguous")
-    if q.numel() + k.numel() == 0:
+    if q_out.numel() + k_out.numel() == 0:
         return q_out, k_out
-    strides = [(ctypes.c_int64 * 3)(*t.stride()[:3]) for t in (q, k, q_out, k_out)]
-    with torch.cuda.device(q.device):
-        native.call("lq_qk_norm_rope", q.data_ptr(), k.data_ptr(), strides[0], strides[1], q_out.data_ptr(),
-                    k_out.data_ptr(), strides[2], strides[3], native.DTYPE_ID[q.dtype], batch, tokens, heads,
-                    k.shape[2], dim, native.ptr(q_weight), native.ptr(k_weight), eps, cos.data_ptr(), sin.data_ptr(),
-                    cos.shape[0], rot, int(interleaved), positions.data_ptr(), positions.stride(0),
-                    positions.stride(1), 1, native.stream_ptr(q.device))
+    native.launch("lq_qk_norm_rope", device.index, q.data_ptr(), k.data_ptr(), native.int64s(qs), native.int64s(ks),
+                  q_out.data_ptr(), k_out.data_ptr(), native.int64s(q_out.stride()), native.int64s(k_out.stride()),
+                  native.DTYPE_ID[dtype], batch, tokens, heads, k_shape[2], dim, wq, wk, eps, cos.data_ptr(),
+                  sin.data_ptr(), table_len, rot, int(interleaved), positions.data_ptr(), *positions.stride(), 1)
     return q_out, k_out

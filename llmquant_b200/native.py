@@ -168,6 +168,35 @@ def stream_ptr(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+# The two questions a call of a few microseconds cannot afford to ask through torch.cuda's objects
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: stream_ptr(index))
+
+
+@functools.lru_cache(maxsize=None)
+def entry(name: str):
+    """The entry point `name` of the library."""
+    return getattr(library(), name)
+
+
+def launch(name: str, index: int, *args):
+    """Invoke one entry point on CUDA device `index` and torch's current stream of it (the stream is the
+    last argument), and raise on a non-zero status."""
+    if _current_device() == index:
+        status = entry(name)(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = entry(name)(*args, _raw_stream(index))
+    if status:
+        check(status)
+
+
+@functools.lru_cache(maxsize=4096)
+def int64s(values):
+    """A C array of int64 (element strides, say); never written to."""
+    return (ctypes.c_int64 * len(values))(*values)
+
+
 def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 

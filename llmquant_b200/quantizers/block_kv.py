@@ -78,6 +78,7 @@ class BlockKVStore:
                               k_ring.data_ptr(), v_ring.data_ptr(), table.data_ptr(), pages, blocks, batch, heads, dim,
                               block, native.DTYPE_ID[self.dtype])
         self._desc, self._ref = desc, ctypes.byref(desc)
+        self._index, self._batch_shape = self.device.index, (batch,)
         self._scratch_bytes = {}
 
     @classmethod
@@ -96,32 +97,25 @@ class BlockKVStore:
     def _span(self, start, count, tokens):
         """(start_dev, start_stride, start, count_dev) of the C calls."""
         if isinstance(start, torch.Tensor):
-            if start.dtype != torch.int64 or start.device != self.device or start.dim() != 1 or \
-                    start.shape[0] not in (1, self.batch):
+            shape = start.shape
+            if start.dtype is not torch.int64 or start.device != self.device or (shape != self._batch_shape and shape != (1,)):
                 raise RuntimeError(f"start must be an int or int64 [{self.batch}] (or [1]) on {self.device}")
-            span = (start.data_ptr(), start.stride(0) if start.shape[0] == self.batch else 0, 0)
+            where, step, start = start.data_ptr(), start.stride(0) if shape == self._batch_shape else 0, 0
         else:
             if not 0 <= start <= self.capacity - (tokens if count is None else 0):
                 raise RuntimeError(f"tokens {start} .. {start + tokens} do not fit a cache of {self.capacity}")
-            span = (0, 0, start)
+            where = step = 0
         if count is None:
-            return (*span, 0)
-        if not isinstance(count, torch.Tensor) or count.dtype != torch.int64 or count.device != self.device or \
-                count.shape != (self.batch,) or not count.is_contiguous():
+            return where, step, start, 0
+        if not isinstance(count, torch.Tensor) or count.dtype is not torch.int64 or count.device != self.device or \
+                count.shape != self._batch_shape or not count.is_contiguous():
             raise RuntimeError(f"count must be None or a contiguous int64 [{self.batch}] on {self.device}")
-        return (*span, count.data_ptr())
-
-    def _call(self, name, *args):
-        if torch.cuda.current_device() == self.device.index:
-            native.call(name, self._ref, *args, native.stream_ptr(self.device))
-        else:
-            with torch.cuda.device(self.device):
-                native.call(name, self._ref, *args, native.stream_ptr(self.device))
+        return where, step, start, count.data_ptr()
 
     def _rows(self, t, name, shape):
-        if t.dtype != self.dtype or t.device != self.device:
+        if t.dtype is not self.dtype or t.device != self.device:
             raise RuntimeError(f"{name} must be {self.dtype} on {self.device}, got {t.dtype} on {t.device}")
-        if tuple(t.shape) != shape:
+        if t.shape != shape:
             raise RuntimeError(f"{name} must be {shape}, got {tuple(t.shape)}")
 
     def append(self, k, v, start, count=None, pdl=True):
@@ -135,10 +129,15 @@ class BlockKVStore:
         span = self._span(start, count, tokens)
         if tokens == 0:
             return
-        k = k if k.stride(3) == 1 else k.contiguous()
-        v = v if v.stride(3) == 1 else v.contiguous()
-        self._call("lq_block_kv_append", k.data_ptr(), v.data_ptr(), (ctypes.c_int64 * 3)(*k.stride()[:3]),
-                   (ctypes.c_int64 * 3)(*v.stride()[:3]), tokens, *span, int(pdl))
+        ks, vs = k.stride(), v.stride()
+        if ks[3] != 1:
+            k = k.contiguous()
+            ks = k.stride()
+        if vs[3] != 1:
+            v = v.contiguous()
+            vs = v.stride()
+        native.launch("lq_block_kv_append", self._index, self._ref, k.data_ptr(), v.data_ptr(), native.int64s(ks),
+                      native.int64s(vs), tokens, *span, int(pdl))
 
     def append_qkv(self, qkv, cos, sin, start, count=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False,
                    q_out=None, pdl=True):
@@ -148,15 +147,18 @@ class BlockKVStore:
         `qk_norm_rope` followed by `append`."""
         if qkv.dim() != 4 or qkv.shape[2] <= 2 * self.heads:
             raise RuntimeError(f"qkv must be [batch, tokens, q heads + {2 * self.heads}, head_dim], got {tuple(qkv.shape)}")
-        tokens, heads = qkv.shape[1], qkv.shape[2] - 2 * self.heads
-        self._rows(qkv, "qkv", (self.batch, tokens, heads + 2 * self.heads, self.head_dim))
-        rot = check_rope_tables(cos, sin, self.device, self.head_dim)
-        check_norm_weights(q_weight, k_weight, self.dtype, self.device, self.head_dim)
-        if isinstance(start, int) and start + tokens > cos.shape[0]:
-            raise RuntimeError(f"tokens {start} .. {start + tokens} have no angles in tables of {cos.shape[0]} positions")
+        _, tokens, heads, _ = qkv.shape
+        self._rows(qkv, "qkv", (self.batch, tokens, heads, self.head_dim))
+        heads -= 2 * self.heads
+        table_len, rot = check_rope_tables(cos, sin, self.device, self.head_dim)
+        wq, wk = check_norm_weights(q_weight, k_weight, self.dtype, self.device, self.head_dim)
+        if isinstance(start, int) and count is None and start + tokens > table_len:
+            raise RuntimeError(f"tokens {start} .. {start + tokens} have no angles in tables of {table_len} positions")
         span = self._span(start, count, tokens)
-        if qkv.stride(3) != 1 or qkv.stride(2) != self.head_dim:
+        strides = qkv.stride()
+        if strides[3] != 1 or strides[2] != self.head_dim:
             qkv = qkv.contiguous()
+            strides = qkv.stride()
         shape = (self.batch, tokens, heads, self.head_dim)
         if q_out is None:
             q_out = torch.empty(shape, dtype=self.dtype, device=self.device)
@@ -166,9 +168,9 @@ class BlockKVStore:
                 raise RuntimeError("q_out must be contiguous")
         if tokens == 0:
             return q_out
-        self._call("lq_block_kv_append_qkv", qkv.data_ptr(), qkv.stride(0), qkv.stride(1), q_out.data_ptr(), heads,
-                   tokens, native.ptr(q_weight), native.ptr(k_weight), eps, cos.data_ptr(), sin.data_ptr(),
-                   cos.shape[0], rot, int(interleaved), *span, int(pdl))
+        native.launch("lq_block_kv_append_qkv", self._index, self._ref, qkv.data_ptr(), strides[0], strides[1],
+                      q_out.data_ptr(), heads, tokens, wq, wk, eps, cos.data_ptr(), sin.data_ptr(), table_len, rot,
+                      int(interleaved), *span, int(pdl))
         return q_out
 
     def scratch_bytes(self, q_heads, tokens):
@@ -176,7 +178,8 @@ class BlockKVStore:
         key = (q_heads, tokens)
         need = self._scratch_bytes.get(key)
         if need is None:
-            need = native.library().lq_block_attn_scratch_bytes(self._ref, q_heads, tokens)
+            with torch.cuda.device(self.device):  # (its SM count decides)
+                need = native.library().lq_block_attn_scratch_bytes(self._ref, q_heads, tokens)
             if need < 0:
                 raise RuntimeError(native.last_error())
             self._scratch_bytes[key] = need
@@ -190,10 +193,10 @@ class BlockKVStore:
         overlap must not share one."""
         if q.dim() != 4:
             raise RuntimeError(f"q must be [batch, tokens, q heads, head_dim], got {tuple(q.shape)}")
-        tokens, heads = q.shape[1], q.shape[2]
+        _, tokens, heads, _ = q.shape
         shape = (self.batch, tokens, heads, self.head_dim)
         self._rows(q, "q", shape)
-        if self.dtype == torch.float32:
+        if self.dtype is torch.float32:
             raise RuntimeError("attention over the block-scaled cache is built for float16 and bfloat16 rows")
         if heads == 0 or heads % self.heads:
             raise RuntimeError(f"{heads} query heads do not share {self.heads} KV heads evenly")
@@ -206,17 +209,19 @@ class BlockKVStore:
                 raise RuntimeError("out must be contiguous")
         if tokens == 0:
             return out
-        if q.stride(3) != 1:
+        strides = q.stride()
+        if strides[3] != 1:
             q = q.contiguous()
+            strides = q.stride()
         need = self.scratch_bytes(heads, tokens)
         if scratch is None:
             scratch = torch.empty(need, dtype=torch.uint8, device=self.device)
-        elif scratch.device != self.device or scratch.dtype != torch.uint8 or scratch.numel() < need or \
+        elif scratch.device != self.device or scratch.dtype is not torch.uint8 or scratch.numel() < need or \
                 not scratch.is_contiguous():
             raise RuntimeError(f"scratch must be {need} contiguous uint8 on {self.device}")
-        scaling = self.head_dim ** -0.5 if scaling is None else scaling
-        self._call("lq_block_attn", q.data_ptr(), (ctypes.c_int64 * 3)(*q.stride()[:3]), out.data_ptr(),
-                   scratch.data_ptr(), need, heads, tokens, *span, scaling, int(pdl))
+        native.launch("lq_block_attn", self._index, self._ref, q.data_ptr(), native.int64s(strides), out.data_ptr(),
+                      scratch.data_ptr(), need, heads, tokens, *span,
+                      self.head_dim ** -0.5 if scaling is None else scaling, int(pdl))
         return out
 
     def read(self, length, start, count=None, tokens=0):
@@ -231,7 +236,7 @@ class BlockKVStore:
         k = torch.empty(shape, dtype=self.dtype, device=self.device)
         v = torch.empty(shape, dtype=self.dtype, device=self.device)
         if length:
-            self._call("lq_block_kv_read", k.data_ptr(), v.data_ptr(), length, *span, tokens, 1)
+            native.launch("lq_block_kv_read", self._index, self._ref, k.data_ptr(), v.data_ptr(), length, *span, tokens, 1)
         return k, v
 
     def check_device_errors(self):
