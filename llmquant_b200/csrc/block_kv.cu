@@ -163,14 +163,14 @@ __device__ __forceinline__ void turn(float& p, float& q, float c, float s) {
 // the warp call this together. fp32 throughout, every operation named, so that the joined and the
 // separate forms round alike; the caller rounds once.
 template <int GRP>
-__device__ __forceinline__ void norm_rope8(float (&x)[8], int D, const float* w, const Rope& rp, const Angles& a) {
+__device__ __forceinline__ void norm_rope8(float (&x)[8], float inv_D, const float* w, const Rope& rp, const Angles& a) {
   if (w != nullptr) {
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ss = __fmaf_rn(x[i], x[i], ss);
 #pragma unroll
     for (int o = GRP / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float r = rsqrtf(__fadd_rn(__fdiv_rn(ss, (float)D), rp.eps));
+    const float r = rsqrtf(__fmaf_rn(ss, inv_D, rp.eps));
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], r), w[i]);
   }
@@ -195,66 +195,63 @@ struct NormRopeArgs {
   const int64_t* positions;
   int64_t ps[2];
   const T *q_weight, *k_weight;
-  int B, T_new, Hq, Hk, D, heads_per_item, items_per_token;
+  int B, T_new, Hq, Hk, D, heads_per_item, q_items, k_items;  // items: lane groups for the heads of a token
 };
 
-// A group of GRP lanes owns one token and up to heads_per_item of its heads: the token's angles
-// are loaded once and stay in registers. Bound by HBM (each value read and written once).
+// A group of GRP lanes owns one token and up to heads_per_item of its query heads, or of its key heads:
+// the token's angles and the weights are loaded once and stay in registers. Bound by HBM (each
+// value read and written once).
 template <typename T, int GRP, bool VEC>
 __global__ void __launch_bounds__(kThreads, 3)
 qk_norm_rope_kernel(const NormRopeArgs<T> p, const Rope rp, int* error_word) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int li = threadIdx.x % GRP;
-  const int64_t items = (int64_t)p.B * p.T_new * p.items_per_token;
+  const int li = threadIdx.x % GRP, each = p.q_items + p.k_items;
+  const int64_t items = (int64_t)p.B * p.T_new * each;
   const int64_t item0 = (int64_t)blockIdx.x * (kThreads / GRP) + threadIdx.x / GRP;
   const bool live = item0 < items;
   const int64_t item = live ? item0 : items - 1;
-  const int64_t token = item / p.items_per_token;
-  const int chunk = (int)(item - token * p.items_per_token);
+  const int64_t token = item / each;
+  const int chunk = (int)(item - token * each);
   const int b = (int)(token / p.T_new), t = (int)(token - (int64_t)b * p.T_new);
+  const bool key = chunk >= p.q_items;
+  const int lo = (key ? chunk - p.q_items : chunk) * p.heads_per_item;
+  const bool mine = live && li * 8 < p.D;
+  const int n = mine ? min(p.heads_per_item, (key ? p.Hk : p.Hq) - lo) : 0;
+  const Hold own = mine ? hold_of(li, rp) : Hold{0, 4};
+  const int step = (int)(key ? p.ks[2] : p.qs[2]), out_step = (int)(key ? p.kos[2] : p.qos[2]);
+  const T* src = (key ? p.k + b * p.ks[0] + t * p.ks[1] + lo * p.ks[2] : p.q + b * p.qs[0] + t * p.qs[1] + lo * p.qs[2]);
+  T* dst = (key ? p.k_out + b * p.kos[0] + t * p.kos[1] + lo * p.kos[2] : p.q_out + b * p.qos[0] + t * p.qos[1] + lo * p.qos[2]);
+  constexpr int UN = 4;  // heads on their way at once
+  Pack8<T> in[UN];
+  auto fetch = [&](int h0) {
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      in[u] = zeros8<T>();
+      if (h0 + u < n) in[u] = load44(src + (h0 + u) * step, own.a, own.b, VEC);
+    }
+  };
+  fetch(0);  // (before the position and the angles that wait for it)
   const int64_t at = p.positions[b * p.ps[0] + t * p.ps[1]];
   const bool known = at >= 0 && at < rp.table_len;
   if (!known && live && li == 0) atomicExch(error_word, LQ_BLOCK_BAD_ANGLE);
-  const int lo = chunk * p.heads_per_item, hi = min(lo + p.heads_per_item, p.Hq + p.Hk);
-  const bool mine = live && li * 8 < p.D;
-  const Hold own = mine ? hold_of(li, rp) : Hold{0, 4};
-  const Angles a = angles_of(rp, known ? at : 0, mine ? li : 32);
-  const T* q = p.q + b * p.qs[0] + t * p.qs[1];
-  const T* k = p.k + b * p.ks[0] + t * p.ks[1];
-  T* q_out = p.q_out + b * p.qos[0] + t * p.qos[1];
-  T* k_out = p.k_out + b * p.kos[0] + t * p.kos[1];
-  constexpr int UN = 4;  // heads on their way at once
-  float w[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  int held = -1;  // whose weights are in w: 0 queries', 1 keys'
+  const T* weight = key ? p.k_weight : p.q_weight;
+  Pack8<T> w = zeros8<T>();
+  if (weight != nullptr && mine) w = load44(weight, own.a, own.b, VEC);
+  Angles a = angles_of(rp, known ? at : 0, mine ? li : 32);
+  if (!known) a.c = a.s = make_float4(NAN, NAN, NAN, NAN);  // no angle: nothing usable
+  const float inv_D = 1.f / p.D;
 #pragma unroll 1
-  for (int h0 = lo; h0 < lo + p.heads_per_item; h0 += UN) {  // (the same trip count for the whole warp)
-    Pack8<T> in[UN];
+  for (int h0 = 0; h0 < p.heads_per_item; h0 += UN) {  // (the same trip count for the whole warp)
+    if (h0 > 0) fetch(h0);
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-      const int h = h0 + u;
-      in[u] = zeros8<T>();
-      if (mine && h < hi) in[u] = load44(h < p.Hq ? q + h * p.qs[2] : k + (h - p.Hq) * p.ks[2], own.a, own.b, VEC);
-    }
-#pragma unroll
-    for (int u = 0; u < UN; ++u) {
-      const int h = h0 + u;
-      if (u >= p.heads_per_item) break;
-      const int whose = h < p.Hq ? 0 : 1;
-      if (p.q_weight != nullptr && whose != held && mine) {
-        unpack8(load44(whose ? p.k_weight : p.q_weight, own.a, own.b, VEC), w);
-        held = whose;
-      }
-      float x[8];
+      if (h0 + u >= p.heads_per_item) break;
+      float x[8], wf[8];
       unpack8(in[u], x);
-      norm_rope8<GRP>(x, p.D, p.q_weight != nullptr ? w : nullptr, rp, a);
-      if (mine && h < hi) {
-        if (!known) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = __int_as_float(0x7fffffff);  // no angle: nothing usable
-        }
-        store44(h < p.Hq ? q_out + h * p.qos[2] : k_out + (h - p.Hq) * p.kos[2], own.a, own.b, pack8<T>(x), VEC);
-      }
+      unpack8(w, wf);
+      norm_rope8<GRP>(x, inv_D, weight != nullptr ? wf : nullptr, rp, a);
+      if (h0 + u < n) store44(dst + (h0 + u) * out_step, own.a, own.b, pack8<T>(x), VEC);
     }
   }
 }
@@ -300,24 +297,19 @@ struct Largest<__nv_bfloat16> : LargestPair<__nv_bfloat162> {
   __device__ __forceinline__ float value() const { return LargestPair::value(__low2float(top), __high2float(top)); }
 };
 
-// Codes of 8 values: rint(x / scale) with IEEE division. x * (1 / scale) is within 2e-5 of the quotient
-// (magnitudes up to 127, three roundings of 2^-24), so its rounding is the quotient's unless it lies
-// that near to a half; then, one value in some thousands, the division itself decides. Adding
-// 1.5 * 2^23 rounds to the nearest even integer and leaves it in the low byte. |x| <= 127 scale
-// up to rounding, so there is nothing to clamp.
+// Codes of 8 values: rint(x / scale), the quotient rounded as IEEE division rounds it (many values lie on
+// a half exactly, so a product with 1 / scale alone would decide wrongly). With inv = 1 / scale
+// correctly rounded, one correction of x * inv by its exact remainder is the correctly rounded
+// quotient (P. Markstein, IBM J. Res. Dev. 34, 1990, theorem 8.1); where the remainder underflows the
+// quotient rounds to zero anyway. Adding 1.5 * 2^23 then rounds to the nearest even integer and
+// leaves it in the low byte. |x| <= 127 scale up to rounding, so there is nothing to clamp.
 __device__ __forceinline__ uint2 codes8(const float (&x)[8], float scale, float inv) {
-  constexpr float kMagic = 12582912.f;
   uint32_t q[8];
-  float worst = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float r = __fmaf_rn(x[i], inv, kMagic);
-    q[i] = __float_as_uint(r);
-    worst = fmaxf(worst, fabsf(__fmaf_rn(x[i], inv, -__fsub_rn(r, kMagic))));
-  }
-  if (worst > 0.4998f) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = (uint32_t)(int)code_of(x[i], scale, -128.f, 127.f);
+    const float near = __fmul_rn(x[i], inv);
+    const float quotient = __fmaf_rn(__fmaf_rn(-near, scale, x[i]), inv, near);
+    q[i] = __float_as_uint(__fadd_rn(quotient, 12582912.f));
   }
   const uint32_t lo = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
   const uint32_t hi = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
@@ -380,7 +372,7 @@ block_append_kernel(const lq_block_kv c, const BlockSpan sp, const AppendArgs<T>
       float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (fresh) unpack8(load44(p.q + b * p.qs[0] + h * p.qs[1] + t * p.qs[2], own.a, own.b, p.vec), x);
       const Angles a = angles_of(rp, fresh && known ? pos : 0, li);
-      norm_rope8<LPR>(x, D, weight != nullptr ? w : nullptr, rp, a);
+      norm_rope8<LPR>(x, 1.f / D, weight != nullptr ? w : nullptr, rp, a);
       if (fresh && !known) {
         if (li == 0) atomicExch(error_word, LQ_BLOCK_BAD_ANGLE);
 #pragma unroll
@@ -423,7 +415,7 @@ block_append_kernel(const lq_block_kv c, const BlockSpan sp, const AppendArgs<T>
       unpack8(r, x);
       const bool known = pos < rp.table_len;
       const Angles a = angles_of(rp, fresh && known ? pos : 0, li);
-      norm_rope8<LPR>(x, D, weight != nullptr ? w : nullptr, rp, a);
+      norm_rope8<LPR>(x, 1.f / D, weight != nullptr ? w : nullptr, rp, a);
       if (fresh && !known) {
         if (li == 0) atomicExch(error_word, LQ_BLOCK_BAD_ANGLE);
 #pragma unroll
@@ -438,18 +430,34 @@ block_append_kernel(const lq_block_kv c, const BlockSpan sp, const AppendArgs<T>
   const int pieces = P * LPR;
   Pack8<T> val[kMaxVec];
   Largest<T> top;
+  constexpr int kStep = kThreads / LPR;  // rows between two pieces of a thread
+  const int row0 = tid / LPR;
+  if (complete && j * P >= s.start && !to_ring) {  // the inside of a long prompt: nothing but new rows to codes
+    const T* row = src + (int64_t)(j * P + row0 - s.start) * step;
 #pragma unroll
-  for (int v = 0; v < kMaxVec; ++v) {
-    if (v * kThreads < pieces) {
-      const int idx = tid + v * kThreads;
-      const int row = idx / LPR, pos = j * P + row;
-      const bool inside = idx < pieces;
-      const bool fresh = inside && pos >= s.start && pos < L;
-      T* held = ring + (int64_t)(pos & (2 * P - 1)) * D;
-      val[v] = fetch(pos, fresh);
-      if (inside && complete && pos < s.start) val[v] = row_load(held, true);
-      if (fresh && to_ring) row_store(held, val[v]);
-      if (complete) top.take(val[v]);
+    for (int v = 0; v < kMaxVec; ++v) {
+      if (v * kThreads < pieces) {
+        val[v] = turned ? fetch(j * P + row0 + v * kStep, row0 + v * kStep < P)
+                        : (row0 + v * kStep < P ? row_load(row, p.vec) : zeros8<T>());
+        row += kStep * step;
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < kMaxVec; ++v)
+      if (v * kThreads < pieces) top.take(val[v]);
+  } else {
+#pragma unroll
+    for (int v = 0; v < kMaxVec; ++v) {
+      if (v * kThreads < pieces) {
+        const int idx = tid + v * kThreads, pos = j * P + row0 + v * kStep;
+        const bool inside = idx < pieces;
+        const bool fresh = inside && pos >= s.start && pos < L;
+        T* held = ring + (int64_t)(pos & (2 * P - 1)) * D;
+        val[v] = fetch(pos, fresh);
+        if (inside && complete && pos < s.start) val[v] = row_load(held, true);
+        if (fresh && to_ring) row_store(held, val[v]);
+        if (complete) top.take(val[v]);
+      }
     }
   }
   if (!complete) return;
@@ -698,9 +706,12 @@ extern "C" int lq_qk_norm_rope(const void* q, const void* k, const int64_t* q_st
   // One head to a lane group while that leaves SMs idle; eight once there are rows enough for
   // eight CTAs on every SM: the angles are then loaded once for eight heads.
   const int64_t busy = rows / ((int64_t)sm_count() * 8 * (kThreads / grp));
-  const int per = busy >= 8 ? 8 : busy >= 4 ? 4 : busy >= 2 ? 2 : 1;
-  const int items_per_token = (Hq + Hk + per - 1) / per;
-  const int64_t groups = (int64_t)B * T_new * items_per_token;
+  int64_t widest = 0;  // (heads of a group are addressed by 32-bit offsets)
+  for (const int64_t v : {Hq ? q_strides[2] : 0, Hk ? k_strides[2] : 0, Hq ? q_out_strides[2] : 0, Hk ? k_out_strides[2] : 0})
+    widest = v > widest ? v : -v > widest ? -v : widest;
+  const int per = widest > 0x7fffffffLL / 8 ? 1 : busy >= 8 ? 8 : busy >= 4 ? 4 : busy >= 2 ? 2 : 1;
+  const int q_items = (Hq + per - 1) / per, k_items = (Hk + per - 1) / per;
+  const int64_t groups = (int64_t)B * T_new * (q_items + k_items);
   const int64_t ctas = (groups + kThreads / grp - 1) / (kThreads / grp);
   LQ_REQUIRE(ctas <= 0x7fffffffLL, LQ_ERR_ARG, "too many rows for one launch");
 #define LQ_GRP(G)                                                                             \
@@ -719,9 +730,9 @@ extern "C" int lq_qk_norm_rope(const void* q, const void* k, const int64_t* q_st
           aligned_rows(q_out, p.qos, 3, sizeof(T)) && aligned_rows(k_out, p.kos, 3, sizeof(T)) &&
           ((uintptr_t)q_weight | (uintptr_t)k_weight) % 16 == 0;
     p.positions = positions; p.ps[0] = pos_stride_b; p.ps[1] = pos_stride_t;
-    p.q_weight = (const T*)(Hq ? q_weight : k_weight); p.k_weight = (const T*)k_weight;
+    p.q_weight = (const T*)q_weight; p.k_weight = (const T*)k_weight;
     p.B = B; p.T_new = T_new; p.Hq = Hq; p.Hk = Hk; p.D = D;
-    p.heads_per_item = per; p.items_per_token = items_per_token;
+    p.heads_per_item = per; p.q_items = q_items; p.k_items = k_items;
     const dim3 grid((unsigned)ctas);
     const cudaStream_t s = (cudaStream_t)stream;
     const char* what = "lq_qk_norm_rope";
