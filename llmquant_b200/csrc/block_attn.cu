@@ -90,7 +90,8 @@ constexpr int kFirst = LQ_S0;  // per cent of a long line that the warps which r
 struct Shape {
   int Hq, G, rows, tile;  // query rows per KV head: T_new * G; rows of one pass
   uint64_t inv_G;         // ceil(2^32 / G): (row * inv_G) >> 32 = row / G for row * G < 2^32
-  int slots, waves;       // warps of a tile's line that run at once; 2: a second wave for long lines
+  int unit_log2;          // tokens of a unit
+  int slots, waves;       // workers of a tile's line that run at once; 2: a second wave for long lines
   uint32_t step;          // 2^32 / slots
 };
 
@@ -110,8 +111,9 @@ __device__ __forceinline__ Tile tile_of(const lq_block_kv& c, const BlockSpan& s
   const int L = x.s.start + x.s.n;
   x.visible = x.s.start + min(x.s.n, token_of(sh, rt * sh.tile + sh.tile - 1) + 1);
   x.held = L & ~(c.block - 1);
-  x.code_units = (min(x.visible, x.held) + kUnit - 1) / kUnit;
-  x.units = x.code_units + (max(0, x.visible - x.held) + kUnit - 1) / kUnit;
+  const int more = (1 << sh.unit_log2) - 1;
+  x.code_units = (min(x.visible, x.held) + more) >> sh.unit_log2;
+  x.units = x.code_units + ((max(0, x.visible - x.held) + more) >> sh.unit_log2);
   if (x.t_lo >= x.s.n) x.code_units = x.units = 0;
   return x;
 }
@@ -708,6 +710,316 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
   }
 }
 
+// ---------------------------------------------------------------- many query rows
+// Drafts of many heads and prompt chunks: 64 query rows to a CTA of four warps, 16 rows to a warp, and
+// units of 64 tokens. Here the conversion of the codes would be most of the work if every warp did it,
+// so each warp converts 16 of a unit's tokens to fp16 in shared memory, for all; keys and values then
+// come by ldmatrix with the queries as the 16 rows of the MMA. Bound by the rate of mma.sync and of
+// the softmax around it. The weights, scales, masks and parts are the ones of the kernel above.
+#ifndef LQ_RC
+#define LQ_RC 3
+#endif
+constexpr int kRowsTile = 64, kRowsWarps = 4, kRowsUnit = 64, kRowsCtas = LQ_RC;  // CTAs on an SM
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+template <int D>
+struct RowsCfg {
+  static constexpr int kTile = kRowsUnit * D * 2;       // a unit's keys, or values, as fp16
+  static constexpr int kRaw = 2 * 16 * D + 16;          // codes of 16 tokens' keys and values, two scales
+  static constexpr size_t kTotal = 2 * kTile + (size_t)kRowsWarps * 2 * kRaw + kRowsWarps * 16;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * kRowsWarps, kRowsCtas)
+block_attn_rows_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const T* __restrict__ q, int64_t qsb,
+                       int64_t qst, int64_t qsh, int q_vec, T* __restrict__ out, float* __restrict__ part,
+                       float2* __restrict__ part_ml, int2* __restrict__ ends, float qk_scale, int* error_word) {
+  using C = RowsCfg<D>;
+  constexpr int KS = D / 16, NT = kRowsUnit / 8, DT = D / 8, RB = D * 2;  // RB: bytes of an fp16 row
+  extern __shared__ __align__(128) uint8_t smem[];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gid = lane >> 2, q4 = lane & 3;
+  const int rt = blockIdx.y, P = c.block, shift = 31 - __clz(P);
+  const int heads = c.batch * c.kv_heads;
+  const uint32_t k_a = smem_u32(smem), v_a = k_a + C::kTile;
+  const uint32_t raw_a = v_a + C::kTile + warp * 2 * C::kRaw;
+  float4* scale_s = reinterpret_cast<float4*>(smem + 2 * C::kTile + kRowsWarps * 2 * C::kRaw);  // [16 tokens]: ks, log2 vs, 1 / vs
+  // ldmatrix rows of this lane: tokens (lane / 16 * 8 + lane % 8) of K, (lane / 8 % 2 * 8 + lane % 8) of V
+  const uint32_t k_row = k_a + ((lane >> 4) * 8 + (lane & 7)) * RB, v_row = v_a + (((lane >> 3) & 1) * 8 + (lane & 7)) * RB;
+  const int3 run = run_of(c, sp, sh, rt, blockIdx.x);
+  int left = run.x, off = run.z;
+
+#pragma unroll 1
+  for (int b = run.y; left > 0; ++b) {
+    const Tile x = tile_of(c, sp, sh, b, rt);
+    if (off >= x.units * c.kv_heads) {
+      off -= x.units * c.kv_heads;
+      continue;
+    }
+    const int* table = c.table + (int64_t)b * c.max_blocks;
+    const int L = x.s.start + x.s.n, code_end = min(x.visible, x.held);
+    // this thread's query rows: gid and gid + 8 of the warp's sixteen
+    const int row0 = rt * kRowsTile + warp * 16 + gid;
+    int seen[2], tok[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      tok[e] = token_of(sh, row0 + 8 * e);
+      seen[e] = x.s.start + tok[e];
+    }
+    const int warp_first = token_of(sh, rt * kRowsTile + warp * 16), warp_last = token_of(sh, rt * kRowsTile + warp * 16 + 15);
+    const bool idle = rt * kRowsTile + warp * 16 >= sh.rows || warp_first >= x.s.n;  // no row of the warp counts
+#pragma unroll 1
+    for (int h = off / x.units; h < c.kv_heads && left > 0; ++h) {
+      const int ua = off - h * x.units;
+      const int ub = min(x.units, ua + left);
+      off += ub - ua;
+      left -= ub - ua;
+      const int last_code = min(ub, x.code_units);
+
+      // codes of this warp's 16 tokens of a unit, on their way while the unit before is multiplied
+      auto issue = [&](int u) {
+        const int pos = u * kRowsUnit + warp * 16;
+        if (u < last_code && pos < code_end) {
+          const uint32_t dst = raw_a + (u & 1) * C::kRaw;
+          const int id = table[pos >> shift];
+          if (id < 0 || id >= c.num_pages) {
+            if (lane == 0) atomicExch(error_word, LQ_BLOCK_BAD_PAGE);
+            if (lane < 2) asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst + 32 * D + lane * 4), "r"(0x7fffffff) : "memory");
+          } else {
+            const int ph = id * c.kv_heads + h;
+            const int64_t at = (((int64_t)ph << shift) + (pos & (P - 1))) * D + lane * 16;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+              cp_async16(dst + (i * 32 + lane) * 16, c.k_pages + at + i * 512);
+              cp_async16(dst + 16 * D + (i * 32 + lane) * 16, c.v_pages + at + i * 512);
+            }
+            if (lane < 2) cp_async4(dst + 32 * D + lane * 4, (lane ? c.v_scales : c.k_scales) + ph);
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      issue(ua);
+
+      // ---- the query rows as A operands, each lifted by a power of two
+      uint32_t qa[KS][4];
+      float qu[2];
+      {
+        uint32_t raw[2][2 * KS];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = row0 + 8 * e, g = row - tok[e] * sh.G;
+          const bool live = row < sh.rows && tok[e] < x.s.n;
+          const uint16_t* p = reinterpret_cast<const uint16_t*>(q) + b * qsb + tok[e] * qst + (int64_t)(h * sh.G + g) * qsh + q4 * 2;
+#pragma unroll
+          for (int k = 0; k < 2 * KS; ++k) {
+            raw[e][k] = 0u;
+            if (live) raw[e][k] = q_vec ? *reinterpret_cast<const uint32_t*>(p + 8 * k) : (uint32_t)p[8 * k] | (uint32_t)p[8 * k + 1] << 16;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float amax = largest_of<T>(raw[e]);
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+          float unit;
+          const float lift = lift_of(finite_abs(amax), 10, unit);
+          qu[e] = amax <= 3.402823466e38f ? unit * qk_scale : __int_as_float(0x7fffffff);
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float2 v = pair_of<T>(raw[e][2 * k + i]);
+              qa[k][e + 2 * i] = as_u32(__floats2half2_rn(v.x * lift, v.y * lift));
+            }
+        }
+      }
+      float o[DT][4], m[2] = {kNone, kNone}, l[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < DT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+
+#pragma unroll 1
+      for (int u = ua; u < ub; ++u) {
+        const bool tail = u >= x.code_units;
+        const int pos0 = tail ? x.held + (u - x.code_units) * kRowsUnit : u * kRowsUnit, mine = pos0 + warp * 16;
+        const int end = tail ? L : code_end;  // positions that exist
+        issue(u + 1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncthreads();  // every warp is done with the unit before (and this lane's codes are there for its warp)
+        const uint32_t k_to = k_a + warp * 16 * RB, v_to = v_a + warp * 16 * RB;
+        if (!tail) {
+          const uint32_t from = raw_a + (u & 1) * C::kRaw;
+          const bool there = mine < code_end;
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            // (a lane's two pieces in the order that keeps eight lanes on different banks)
+            const int idx = i * 32 + lane, row = idx / (D / 16), chunk = idx % (D / 16) * 2, odd = D == 128 ? (lane >> 2) & 1 : 0;
+            const uint32_t to0 = row * RB + (((chunk + odd) ^ (row & 7)) << 4), to1 = row * RB + (((chunk + 1 - odd) ^ (row & 7)) << 4);
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+              uint4 w = make_uint4(0u, 0u, 0u, 0u);  // (nothing there: the weights are zero, the values must be numbers)
+              if (there) w = lds128m(from + kv * 16 * D + idx * 16);
+              const uint32_t a = (odd ? w.z : w.x) ^ 0x80808080u, b2 = (odd ? w.w : w.y) ^ 0x80808080u;
+              const uint32_t c2 = (odd ? w.x : w.z) ^ 0x80808080u, d2 = (odd ? w.y : w.w) ^ 0x80808080u;
+              sts128((kv ? v_to : k_to) + to0, codes_h2(a, 0x4140u), codes_h2(a, 0x4342u), codes_h2(b2, 0x4140u), codes_h2(b2, 0x4342u));
+              sts128((kv ? v_to : k_to) + to1, codes_h2(c2, 0x4140u), codes_h2(c2, 0x4342u), codes_h2(d2, 0x4140u), codes_h2(d2, 0x4342u));
+            }
+          }
+          if (lane == 0) {
+            const uint2 sc = lds64(from + 32 * D);
+            const float vs = there ? __uint_as_float(sc.y) : 1.f;
+            scale_s[warp] = make_float4(there ? __uint_as_float(sc.x) : 1.f, log2_of(vs), fminf(inverse_of(vs), 3.0e38f), 0.f);
+          }
+        } else {
+          // rows of the incomplete block: a lane takes half a row, lifted by a power of two of the 16 rows
+          const int pos = mine + (lane >> 1);
+          const int64_t row = (((int64_t)b * c.kv_heads + h) * 2 * P + (pos & (2 * P - 1))) * D + (lane & 1) * (D / 2);
+          float unit[2];
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(kv ? c.v_ring : c.k_ring) + row);
+            float top = 0.f;
+#pragma unroll 1
+            for (int i = 0; i < D / 16; ++i) {
+              const uint4 v = pos < L ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+              const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float2 p = pair_of<T>(w[k]);
+                top = fmaxf(top, fmaxf(finite_abs(p.x), finite_abs(p.y)));
+              }
+            }
+            const float lift = lift_of(warp_max(top), kv ? 7 : 10, unit[kv]);
+            const int r = lane >> 1;
+#pragma unroll 1
+            for (int i = 0; i < D / 16; ++i) {  // (read again from L1)
+              const uint4 v = pos < L ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+              const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+              uint32_t z[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float2 p = pair_of<T>(w[k]);
+                z[k] = as_u32(__floats2half2_rn(p.x * lift, p.y * lift));
+              }
+              const int chunk = (lane & 1) * (D / 16) + i;
+              sts128((kv ? v_to : k_to) + r * RB + ((chunk ^ (r & 7)) << 4), z[0], z[1], z[2], z[3]);
+            }
+          }
+          if (lane == 0) scale_s[warp] = make_float4(unit[0], log2_of(unit[1]), inverse_of(unit[1]), 0.f);
+        }
+        __syncthreads();
+        if (idle || pos0 > x.s.start + min(warp_last, x.s.n - 1)) continue;  // none of the warp's rows sees the unit
+
+        // ---- scores of 16 rows and 64 tokens
+        float acc[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int j = 0; j < NT; j += 2) {
+            uint32_t w[4];
+            ldmatrix4(w, k_row + j * 8 * RB + (((2 * k + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
+            mma16(acc[j], qa[k][0], qa[k][1], qa[k][2], qa[k][3], w[0], w[1]);
+            mma16(acc[j + 1], qa[k][0], qa[k][1], qa[k][2], qa[k][3], w[2], w[3]);
+          }
+        const bool masked = pos0 + kRowsUnit - 1 > min(x.s.start + warp_first, end - 1);
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const float4 sc = scale_s[j >> 1];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            acc[j][i] = fmaf(acc[j][i], qu[i >> 1] * sc.x, sc.y);
+            if (masked) {
+              const int pos = pos0 + j * 8 + q4 * 2 + (i & 1);
+              if (pos > seen[i >> 1] || pos >= end) acc[j][i] = -INFINITY;
+            }
+            mx[i >> 1] = fmaxf(mx[i >> 1], acc[j][i]);
+          }
+        }
+        if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f)) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float to = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+            to = fmaxf(fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 2)), m[e]);
+            const float corr = exp2_of(m[e] - to);
+            m[e] = to;
+            l[e] *= corr;
+#pragma unroll
+            for (int i = 0; i < DT; ++i) {
+              o[i][2 * e] *= corr;
+              o[i][2 * e + 1] *= corr;
+            }
+          }
+        }
+        uint32_t pa[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const float inv = scale_s[j >> 1].z;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float w0 = exp2_of(acc[j][2 * e] - m[e]), w1 = exp2_of(acc[j][2 * e + 1] - m[e]);
+            l[e] = fmaf(w0 + w1, inv, l[e]);
+            pa[j][e] = as_u32(__floats2half2_rn(w0, w1));
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < NT / 2; ++k)
+#pragma unroll
+          for (int d = 0; d < DT; d += 2) {
+            uint32_t w[4];
+            ldmatrix4_trans(w, v_row + k * 16 * RB + (((d + (lane >> 4)) ^ (lane & 7)) << 4));
+            mma16(o[d], pa[2 * k][0], pa[2 * k][1], pa[2 * k + 1][0], pa[2 * k + 1][1], w[0], w[1]);
+            mma16(o[d + 1], pa[2 * k][0], pa[2 * k][1], pa[2 * k + 1][0], pa[2 * k + 1][1], w[2], w[3]);
+          }
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+      // ---- what this run has of the (sequence, head): all of it, or a part
+      const bool whole = ua == 0 && ub == x.units;
+      const int64_t slot = ((int64_t)rt * (gridDim.x + heads) + blockIdx.x + b * c.kv_heads + h) * kRowsTile;
+      if (threadIdx.x == 0) {  // for the join: the runs that begin and end it
+        if (ua == 0) ends[(int64_t)rt * heads + b * c.kv_heads + h].x = blockIdx.x;
+        if (ub == x.units) ends[(int64_t)rt * heads + b * c.kv_heads + h].y = blockIdx.x;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[e];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        const int row = row0 + 8 * e, r = warp * 16 + gid + 8 * e, g = row - tok[e] * sh.G;
+        if (row >= sh.rows) continue;
+        if (whole) {
+          const bool live = tok[e] < x.s.n;
+          const float inv = live ? 1.f / sum : 0.f;
+          uint32_t* dst = reinterpret_cast<uint32_t*>(out + (((int64_t)b * sp.tokens + tok[e]) * sh.Hq + h * sh.G + g) * D) + q4;
+#pragma unroll
+          for (int i = 0; i < DT; ++i) dst[4 * i] = live ? pair_to<T>(o[i][2 * e] * inv, o[i][2 * e + 1] * inv) : 0u;
+        } else {
+          float2* dst = reinterpret_cast<float2*>(part + (slot + r) * D) + q4;
+#pragma unroll
+          for (int i = 0; i < DT; ++i) dst[4 * i] = make_float2(o[i][2 * e], o[i][2 * e + 1]);
+          if (q4 == 0) part_ml[slot + r] = make_float2(m[e], sum);
+        }
+      }
+      __syncthreads();  // the shared memory is free for the next (sequence, head)
+    }
+    off -= x.units * c.kv_heads;
+  }
+}
+
 // ---------------------------------------------------------------- join the parts
 // grid (sequences x KV heads, row groups x column groups of a tile, row tiles): an output row that
 // several warps shared is the weighted sum of their parts; one that none took (it does not count)
@@ -800,6 +1112,11 @@ block_attn_join_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
 }
 
 // ---------------------------------------------------------------- host
+#ifndef LQ_ALONE
+#define LQ_ALONE 16
+#endif
+constexpr int kAloneRows = LQ_ALONE;
+
 struct Plan {
   Shape sh;
   int nt, tiles, runs;
@@ -811,10 +1128,13 @@ Plan plan_of(const lq_block_kv& c, int Hq, int T_new) {
   p.sh.G = Hq / c.kv_heads;
   p.sh.rows = T_new * p.sh.G;
   p.sh.inv_G = (0x100000000ULL + p.sh.G - 1) / p.sh.G;
-  p.nt = p.sh.rows <= 8 ? 1 : 2;
-  p.sh.tile = 8 * p.nt;
+  // Up to 16 rows the codes' bytes decide, and warps that work alone stream them best; more rows share
+  // the conversion of a unit.
+  p.nt = p.sh.rows <= 8 ? 1 : p.sh.rows <= kAloneRows ? 2 : 0;
+  p.sh.tile = p.nt ? 8 * p.nt : kRowsTile;
+  p.sh.unit_log2 = p.nt ? 5 : 6;
   p.tiles = (p.sh.rows + p.sh.tile - 1) / p.sh.tile;
-  const int at_once = sm_count() * (p.nt == 2 ? Cfg<128, 2>::kWarps : c.head_dim == 64 ? Cfg<64, 1>::kWarps : Cfg<128, 1>::kWarps);
+  const int at_once = sm_count() * (p.nt == 0 ? kRowsCtas : p.nt == 2 ? Cfg<128, 2>::kWarps : c.head_dim == 64 ? Cfg<64, 1>::kWarps : Cfg<128, 1>::kWarps);
   p.sh.slots = at_once / p.tiles > 1 ? at_once / p.tiles : 2;
   p.sh.step = (uint32_t)(0x100000000ULL / p.sh.slots);
   p.sh.waves = p.tiles == 1 ? 2 : 1;
@@ -863,17 +1183,30 @@ int launch(Kern kern, dim3 grid, int threads, size_t smem, cudaStream_t stream, 
 }
 
 template <typename T, int D, int NT>
+struct Main {
+  static auto kernel() { return block_attn_kernel<T, D, NT>; }
+  static constexpr size_t kSmem = Cfg<D, NT>::kRing;
+  static constexpr int kThreads = 32;
+};
+template <typename T, int D>
+struct Main<T, D, 0> {
+  static auto kernel() { return block_attn_rows_kernel<T, D>; }
+  static constexpr size_t kSmem = RowsCfg<D>::kTotal;
+  static constexpr int kThreads = 32 * kRowsWarps;
+};
+
+template <typename T, int D, int NT>
 int run(const lq_block_kv& c, const BlockSpan& sp, const Plan& p, const void* q, const int64_t* qs, void* out, void* scratch,
         float scaling, int pdl, cudaStream_t stream, int* error_word, const char* what) {
-  auto kern = block_attn_kernel<T, D, NT>;
-  constexpr size_t smem = Cfg<D, NT>::kRing;
+  auto kern = Main<T, D, NT>::kernel();
+  constexpr size_t smem = Main<T, D, NT>::kSmem;
   if (const int rc = ensure_smem_limit(reinterpret_cast<const void*>(kern), (int)smem, what)) return rc;
   const float qk_scale = scaling * 1.4426950408889634f;
   const int q_vec = (((uintptr_t)q | (uintptr_t)(qs[0] * 2) | (uintptr_t)(qs[1] * 2) | (uintptr_t)(qs[2] * 2)) & 15) == 0;
   float* part = (float*)scratch;
   float2* part_ml = (float2*)(part + slots_of(c, p) * D);
   int2* ends = (int2*)(part_ml + slots_of(c, p));
-  if (const int rc = launch(kern, dim3((unsigned)p.runs, (unsigned)p.tiles), 32, smem, stream, pdl, what, c, sp, p.sh,
+  if (const int rc = launch(kern, dim3((unsigned)p.runs, (unsigned)p.tiles), Main<T, D, NT>::kThreads, smem, stream, pdl, what, c, sp, p.sh,
                             (const T*)q, qs[0], qs[1], qs[2], q_vec, (T*)out, part, part_ml, ends, qk_scale,
                             error_word))
     return rc;
@@ -883,8 +1216,8 @@ int run(const lq_block_kv& c, const BlockSpan& sp, const Plan& p, const void* q,
   const int64_t tops = (int64_t)c.batch * c.kv_heads * p.tiles;
   const int rows = p.sh.rows < p.sh.tile ? p.sh.rows : p.sh.tile;
   const bool few = tops * rows <= 2 * sm_count();
-  const int each = few ? 1 : rows, cols = few ? 4 : 1, threads = few ? 512 : 2 * rows * D / 4;
-  return launch(block_attn_join_kernel<T, D>, dim3((unsigned)(c.batch * c.kv_heads), (unsigned)(rows / each * cols), (unsigned)p.tiles),
+  const int each = few ? 1 : rows < 8 ? rows : 8, cols = few ? 4 : 1, threads = few ? 512 : 2 * each * D / 4;
+  return launch(block_attn_join_kernel<T, D>, dim3((unsigned)(c.batch * c.kv_heads), (unsigned)((rows + each - 1) / each * cols), (unsigned)p.tiles),
                 threads, 0, stream, 1, what, c, sp, p.sh, p.runs, each, cols, (T*)out, (const float*)part, (const float2*)part_ml,
                 (const int2*)ends, error_word);
 }
@@ -894,8 +1227,8 @@ int dispatch(const lq_block_kv& c, const BlockSpan& sp, const Plan& p, const voi
              float scaling, int pdl, cudaStream_t stream, int* error_word, const char* what) {
 #define LQ_CASE(DD, NN) \
   if (c.head_dim == DD && p.nt == NN) return run<T, DD, NN>(c, sp, p, q, qs, out, scratch, scaling, pdl, stream, error_word, what);
-  LQ_CASE(64, 1) LQ_CASE(64, 2)
-  LQ_CASE(128, 1) LQ_CASE(128, 2)
+  LQ_CASE(64, 0) LQ_CASE(64, 1) LQ_CASE(64, 2)
+  LQ_CASE(128, 0) LQ_CASE(128, 1) LQ_CASE(128, 2)
 #undef LQ_CASE
   return fail(LQ_ERR_UNSUPPORTED, "%s: no kernel for this shape", what);
 }
