@@ -22,6 +22,7 @@
 #include <type_traits>
 
 #include "block_kv.cuh"
+#include "tcgen05.cuh"
 
 namespace lq {
 namespace {
@@ -711,55 +712,90 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
 }
 
 // ---------------------------------------------------------------- many query rows
-// Drafts of many heads and prompt chunks: 64 query rows to a CTA of four warps, 16 rows to a warp, and
-// units of 64 tokens. Here the conversion of the codes would be most of the work if every warp did it,
-// so each warp converts 16 of a unit's tokens to fp16 in shared memory, for all; keys and values then
-// come by ldmatrix with the queries as the 16 rows of the MMA. Bound by the rate of mma.sync and of
-// the softmax around it. The weights, scales, masks and parts are the ones of the kernel above.
-#ifndef LQ_RC
-#define LQ_RC 3
-#endif
-constexpr int kRowsTile = 64, kRowsWarps = 4, kRowsUnit = 64, kRowsCtas = LQ_RC;  // CTAs on an SM
+// Prompt chunks, and drafts of many heads: 128 query rows to a CTA, one to a thread, and units of 64
+// tokens, on tcgen05. The products' accumulators are in tensor memory: scores [128, 64], outputs
+// [128, D]; a thread reads its row of scores, so that maximum and sum need no exchange, and writes its
+// row of weights as the next product's A operand. The codes become fp16 tiles in shared memory once for
+// all 128 rows, the values' tile transposed on the way (both operands of a product run along k). The
+// outputs are only touched, by a warp for its 32 rows, when a row's maximum rises by 2^8. Two CTAs on an
+// SM: while one converts or exponentiates the other's products run. The weights, scales, masks and
+// parts are the ones of the kernel above. Bound by the instructions around the products, not by them.
+constexpr int kManyTile = 128, kManyThreads = 128, kManyUnit = 64, kManyCtas = 2;  // CTAs on an SM
+constexpr uint32_t kManyCols = 256, kOutCol = 64;  // columns of tensor memory a CTA takes; where the outputs begin
 
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
+template <int D>
+struct ManyCfg {
+  static constexpr int kQ = kManyTile * D * 2, kK = kManyUnit * D * 2, kV = D * kManyUnit * 2, kP = kManyTile * kManyUnit * 2;
+  static constexpr int kRaw = kManyUnit * D;  // a unit's codes of keys, or values
+  static constexpr size_t kTotal = 1024 + kQ + kK + kV + kP + 2 * kRaw;  // (1024: to begin on such a boundary)
+  static_assert(kManyCtas * (kTotal + 1400) <= 228 * 1024, "");
+};
+
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-
-template <int D>
-struct RowsCfg {
-  static constexpr int kTile = kRowsUnit * D * 2;       // a unit's keys, or values, as fp16
-  static constexpr int kRaw = 2 * 16 * D + 16;          // codes of 16 tokens' keys and values, two scales
-  static constexpr size_t kTotal = 2 * kTile + (size_t)kRowsWarps * 2 * kRaw + kRowsWarps * 16;
-};
+__device__ __forceinline__ void sts32(uint32_t addr, uint32_t a) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(a) : "memory");
+}
+// f32 <- f16 x f16 of kind::f16, M = 128, N columns, both operands along k
+constexpr uint32_t many_idesc(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kManyTile >> 4) << 24); }
+// Address of 16-byte piece `piece` of row `row` in a tile of 128-byte rows, 128-byte swizzle
+__device__ __forceinline__ uint32_t swizzled(uint32_t tile, int row, int piece) {
+  return tile + row * 128 + ((piece ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+        "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+        "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
 
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * kRowsWarps, kRowsCtas)
-block_attn_rows_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const T* __restrict__ q, int64_t qsb,
+__global__ void __launch_bounds__(kManyThreads, kManyCtas)
+block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const T* __restrict__ q, int64_t qsb,
                        int64_t qst, int64_t qsh, int q_vec, T* __restrict__ out, float* __restrict__ part,
                        float2* __restrict__ part_ml, int2* __restrict__ ends, float qk_scale, int* error_word) {
-  using C = RowsCfg<D>;
-  constexpr int KS = D / 16, NT = kRowsUnit / 8, DT = D / 8, RB = D * 2;  // RB: bytes of an fp16 row
-  extern __shared__ __align__(128) uint8_t smem[];
+  using C = ManyCfg<D>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ __align__(8) uint64_t bar_s[2];   // scores are there, outputs are there
+  __shared__ uint32_t tmem_s;
+  __shared__ float4 scale_s[4];                // of 16 tokens each: ks, log2 vs, 1 / vs
+  __shared__ float2 raw_scale_s[4], lift_s[4];
+  __shared__ int dead_s;
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t q_a = (smem_u32(smem) + 1023u) & ~1023u, k_a = q_a + C::kQ, v_a = k_a + C::kK, p_a = v_a + C::kV;
+  const uint32_t raw_k = p_a + C::kP, raw_v = raw_k + C::kRaw;
+  const uint32_t bar_scores = smem_u32(&bar_s[0]), bar_outputs = smem_u32(&bar_s[1]);
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&tmem_s)), "r"(kManyCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 0) {
+    mbar_init(bar_scores, 1);
+    mbar_init(bar_outputs, 1);
+    dead_s = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  // (only now: a dependent kernel that takes tensor memory before it waits must not come between)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gid = lane >> 2, q4 = lane & 3;
+  const uint32_t tmem = tmem_s + ((uint32_t)(warp * 32) << 16);  // this warp's rows
   const int rt = blockIdx.y, P = c.block, shift = 31 - __clz(P);
   const int heads = c.batch * c.kv_heads;
-  const uint32_t k_a = smem_u32(smem), v_a = k_a + C::kTile;
-  const uint32_t raw_a = v_a + C::kTile + warp * 2 * C::kRaw;
-  float4* scale_s = reinterpret_cast<float4*>(smem + 2 * C::kTile + kRowsWarps * 2 * C::kRaw);  // [16 tokens]: ks, log2 vs, 1 / vs
-  // ldmatrix rows of this lane: tokens (lane / 16 * 8 + lane % 8) of K, (lane / 8 % 2 * 8 + lane % 8) of V
-  const uint32_t k_row = k_a + ((lane >> 4) * 8 + (lane & 7)) * RB, v_row = v_a + (((lane >> 3) & 1) * 8 + (lane & 7)) * RB;
   const int3 run = run_of(c, sp, sh, rt, blockIdx.x);
   int left = run.x, off = run.z;
+  uint32_t phase = 0;  // of both barriers: one completion of each per unit
+  const int row = rt * kManyTile + tid, tok = token_of(sh, row), g = row - tok * sh.G;
 
 #pragma unroll 1
   for (int b = run.y; left > 0; ++b) {
@@ -769,17 +805,8 @@ block_attn_rows_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
       continue;
     }
     const int* table = c.table + (int64_t)b * c.max_blocks;
-    const int L = x.s.start + x.s.n, code_end = min(x.visible, x.held);
-    // this thread's query rows: gid and gid + 8 of the warp's sixteen
-    const int row0 = rt * kRowsTile + warp * 16 + gid;
-    int seen[2], tok[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      tok[e] = token_of(sh, row0 + 8 * e);
-      seen[e] = x.s.start + tok[e];
-    }
-    const int warp_first = token_of(sh, rt * kRowsTile + warp * 16), warp_last = token_of(sh, rt * kRowsTile + warp * 16 + 15);
-    const bool idle = rt * kRowsTile + warp * 16 >= sh.rows || warp_first >= x.s.n;  // no row of the warp counts
+    const int L = x.s.start + x.s.n, code_end = min(x.visible, x.held), seen = x.s.start + tok;
+    const bool live = row < sh.rows && tok < x.s.n;
 #pragma unroll 1
     for (int h = off / x.units; h < c.kv_heads && left > 0; ++h) {
       const int ua = off - h * x.units;
@@ -788,236 +815,286 @@ block_attn_rows_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
       left -= ub - ua;
       const int last_code = min(ub, x.code_units);
 
-      // codes of this warp's 16 tokens of a unit, on their way while the unit before is multiplied
+      // codes of this warp's 16 tokens of a unit; the values' pieces of a row permuted by its pair of tokens
       auto issue = [&](int u) {
-        const int pos = u * kRowsUnit + warp * 16;
+        const int pos = u * kManyUnit + warp * 16;
         if (u < last_code && pos < code_end) {
-          const uint32_t dst = raw_a + (u & 1) * C::kRaw;
           const int id = table[pos >> shift];
           if (id < 0 || id >= c.num_pages) {
-            if (lane == 0) atomicExch(error_word, LQ_BLOCK_BAD_PAGE);
-            if (lane < 2) asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst + 32 * D + lane * 4), "r"(0x7fffffff) : "memory");
+            if (lane == 0) {
+              atomicExch(error_word, LQ_BLOCK_BAD_PAGE);
+              raw_scale_s[warp] = make_float2(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff));
+            }
           } else {
             const int ph = id * c.kv_heads + h;
-            const int64_t at = (((int64_t)ph << shift) + (pos & (P - 1))) * D + lane * 16;
+            const int64_t at = (((int64_t)ph << shift) + (pos & (P - 1))) * D;
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
-              cp_async16(dst + (i * 32 + lane) * 16, c.k_pages + at + i * 512);
-              cp_async16(dst + 16 * D + (i * 32 + lane) * 16, c.v_pages + at + i * 512);
+              const int idx = i * 32 + lane, r = warp * 16 + idx / (D / 16), piece = idx % (D / 16);
+              cp_async16(raw_k + r * D + piece * 16, c.k_pages + at + idx * 16);
+              cp_async16(raw_v + r * D + ((piece ^ ((r >> 1) & (D / 16 - 1))) << 4), c.v_pages + at + idx * 16);
             }
-            if (lane < 2) cp_async4(dst + 32 * D + lane * 4, (lane ? c.v_scales : c.k_scales) + ph);
+            if (lane < 2) cp_async4(smem_u32(&raw_scale_s[warp]) + lane * 4, (lane ? c.v_scales : c.k_scales) + ph);
           }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
       issue(ua);
 
-      // ---- the query rows as A operands, each lifted by a power of two
-      uint32_t qa[KS][4];
-      float qu[2];
+      // ---- this thread's query row to its row of the A tile, lifted by a power of two
+      float qu;
       {
-        uint32_t raw[2][2 * KS];
+        uint32_t raw[D / 2];
+        load_words(raw, reinterpret_cast<const uint16_t*>(q) + b * qsb + tok * qst + (int64_t)(h * sh.G + g) * qsh, live, q_vec);
+        const float amax = largest_of<T>(raw);
+        float unit;
+        const float lift = lift_of(finite_abs(amax), 10, unit);
+        qu = amax <= 3.402823466e38f ? unit * qk_scale : __int_as_float(0x7fffffff);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int row = row0 + 8 * e, g = row - tok[e] * sh.G;
-          const bool live = row < sh.rows && tok[e] < x.s.n;
-          const uint16_t* p = reinterpret_cast<const uint16_t*>(q) + b * qsb + tok[e] * qst + (int64_t)(h * sh.G + g) * qsh + q4 * 2;
+        for (int i = 0; i < D / 8; ++i) {
+          uint32_t w[4];
 #pragma unroll
-          for (int k = 0; k < 2 * KS; ++k) {
-            raw[e][k] = 0u;
-            if (live) raw[e][k] = q_vec ? *reinterpret_cast<const uint32_t*>(p + 8 * k) : (uint32_t)p[8 * k] | (uint32_t)p[8 * k + 1] << 16;
+          for (int k = 0; k < 4; ++k) {
+            const float2 v = pair_of<T>(raw[4 * i + k]);
+            w[k] = as_u32(__floats2half2_rn(v.x * lift, v.y * lift));
           }
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float amax = largest_of<T>(raw[e]);
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-          float unit;
-          const float lift = lift_of(finite_abs(amax), 10, unit);
-          qu[e] = amax <= 3.402823466e38f ? unit * qk_scale : __int_as_float(0x7fffffff);
-#pragma unroll
-          for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float2 v = pair_of<T>(raw[e][2 * k + i]);
-              qa[k][e + 2 * i] = as_u32(__floats2half2_rn(v.x * lift, v.y * lift));
-            }
+          sts128(swizzled(q_a + (i >> 3) * kManyTile * 128, tid, i & 7), w[0], w[1], w[2], w[3]);
         }
       }
-      float o[DT][4], m[2] = {kNone, kNone}, l[2] = {0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < DT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+      float m = kNone, l = 0.f;
 
 #pragma unroll 1
       for (int u = ua; u < ub; ++u) {
         const bool tail = u >= x.code_units;
-        const int pos0 = tail ? x.held + (u - x.code_units) * kRowsUnit : u * kRowsUnit, mine = pos0 + warp * 16;
+        const int pos0 = tail ? x.held + (u - x.code_units) * kManyUnit : u * kManyUnit, mine = pos0 + warp * 16;
         const int end = tail ? L : code_end;  // positions that exist
-        issue(u + 1);
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-        __syncthreads();  // every warp is done with the unit before (and this lane's codes are there for its warp)
-        const uint32_t k_to = k_a + warp * 16 * RB, v_to = v_a + warp * 16 * RB;
-        if (!tail) {
-          const uint32_t from = raw_a + (u & 1) * C::kRaw;
-          const bool there = mine < code_end;
+        // ---- keys: fp16 tile of the score product (its last reader, the unit before's product, has ended)
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (tail) {  // 16 rows of the ring to a warp: what lifts them
+          const int pos = mine + (lane >> 1);
+          const int64_t at = (((int64_t)b * c.kv_heads + h) * 2 * P + (pos & (2 * P - 1))) * D + (lane & 1) * (D / 2);
+          float top[2] = {0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < D / 32; ++i) {
-            // (a lane's two pieces in the order that keeps eight lanes on different banks)
-            const int idx = i * 32 + lane, row = idx / (D / 16), chunk = idx % (D / 16) * 2, odd = D == 128 ? (lane >> 2) & 1 : 0;
-            const uint32_t to0 = row * RB + (((chunk + odd) ^ (row & 7)) << 4), to1 = row * RB + (((chunk + 1 - odd) ^ (row & 7)) << 4);
+          for (int kv = 0; kv < 2; ++kv)
+#pragma unroll 2
+            for (int i = 0; i < D / 16; ++i) {
+              const uint4 v = pos < L ? reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(kv ? c.v_ring : c.k_ring) + at)[i]
+                                      : make_uint4(0u, 0u, 0u, 0u);
+              const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int kv = 0; kv < 2; ++kv) {
-              uint4 w = make_uint4(0u, 0u, 0u, 0u);  // (nothing there: the weights are zero, the values must be numbers)
-              if (there) w = lds128m(from + kv * 16 * D + idx * 16);
-              const uint32_t a = (odd ? w.z : w.x) ^ 0x80808080u, b2 = (odd ? w.w : w.y) ^ 0x80808080u;
-              const uint32_t c2 = (odd ? w.x : w.z) ^ 0x80808080u, d2 = (odd ? w.y : w.w) ^ 0x80808080u;
-              sts128((kv ? v_to : k_to) + to0, codes_h2(a, 0x4140u), codes_h2(a, 0x4342u), codes_h2(b2, 0x4140u), codes_h2(b2, 0x4342u));
-              sts128((kv ? v_to : k_to) + to1, codes_h2(c2, 0x4140u), codes_h2(c2, 0x4342u), codes_h2(d2, 0x4140u), codes_h2(d2, 0x4342u));
+              for (int k = 0; k < 4; ++k) {
+                const float2 p = pair_of<T>(w[k]);
+                top[kv] = fmaxf(top[kv], fmaxf(finite_abs(p.x), finite_abs(p.y)));
+              }
             }
-          }
+          float unit[2];
+          const float klift = lift_of(warp_max(top[0]), 10, unit[0]), vlift = lift_of(warp_max(top[1]), 7, unit[1]);
           if (lane == 0) {
-            const uint2 sc = lds64(from + 32 * D);
-            const float vs = there ? __uint_as_float(sc.y) : 1.f;
-            scale_s[warp] = make_float4(there ? __uint_as_float(sc.x) : 1.f, log2_of(vs), fminf(inverse_of(vs), 3.0e38f), 0.f);
+            lift_s[warp] = make_float2(klift, vlift);
+            scale_s[warp] = make_float4(unit[0], log2_of(unit[1]), inverse_of(unit[1]), 0.f);
+          }
+#pragma unroll 2
+          for (int i = 0; i < D / 16; ++i) {
+            const uint4 v = pos < L ? reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(c.k_ring) + at)[i] : make_uint4(0u, 0u, 0u, 0u);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            uint32_t z[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 p = pair_of<T>(w[k]);
+              z[k] = as_u32(__floats2half2_rn(p.x * klift, p.y * klift));
+            }
+            const int piece = (lane & 1) * (D / 16) + i;
+            sts128(swizzled(k_a + (piece >> 3) * kManyUnit * 128, warp * 16 + (lane >> 1), piece & 7), z[0], z[1], z[2], z[3]);
           }
         } else {
-          // rows of the incomplete block: a lane takes half a row, lifted by a power of two of the 16 rows
-          const int pos = mine + (lane >> 1);
-          const int64_t row = (((int64_t)b * c.kv_heads + h) * 2 * P + (pos & (2 * P - 1))) * D + (lane & 1) * (D / 2);
-          float unit[2];
+          __syncwarp();
+          const bool there = mine < code_end;
+          // (a lane's two pieces in the order that keeps eight lanes on different banks)
+          const int odd = D == 128 ? (lane >> 2) & 1 : 0;
 #pragma unroll
-          for (int kv = 0; kv < 2; ++kv) {
-            const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(kv ? c.v_ring : c.k_ring) + row);
-            float top = 0.f;
-#pragma unroll 1
-            for (int i = 0; i < D / 16; ++i) {
-              const uint4 v = pos < L ? src[i] : make_uint4(0u, 0u, 0u, 0u);
-              const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float2 p = pair_of<T>(w[k]);
-                top = fmaxf(top, fmaxf(finite_abs(p.x), finite_abs(p.y)));
-              }
-            }
-            const float lift = lift_of(warp_max(top), kv ? 7 : 10, unit[kv]);
-            const int r = lane >> 1;
-#pragma unroll 1
-            for (int i = 0; i < D / 16; ++i) {  // (read again from L1)
-              const uint4 v = pos < L ? src[i] : make_uint4(0u, 0u, 0u, 0u);
-              const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-              uint32_t z[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float2 p = pair_of<T>(w[k]);
-                z[k] = as_u32(__floats2half2_rn(p.x * lift, p.y * lift));
-              }
-              const int chunk = (lane & 1) * (D / 16) + i;
-              sts128((kv ? v_to : k_to) + r * RB + ((chunk ^ (r & 7)) << 4), z[0], z[1], z[2], z[3]);
-            }
+          for (int i = 0; i < D / 32; ++i) {
+            const int idx = i * 32 + lane, r = warp * 16 + idx / (D / 16), piece = idx % (D / 16) * 2;
+            uint4 w = make_uint4(0u, 0u, 0u, 0u);
+            if (there) w = lds128m(raw_k + r * D + (idx % (D / 16)) * 16);
+            const uint32_t a0 = (odd ? w.z : w.x) ^ 0x80808080u, a1 = (odd ? w.w : w.y) ^ 0x80808080u;
+            const uint32_t a2 = (odd ? w.x : w.z) ^ 0x80808080u, a3 = (odd ? w.y : w.w) ^ 0x80808080u;
+            const uint32_t tile = k_a + (piece >> 3) * kManyUnit * 128;
+            sts128(swizzled(tile, r, (piece & 7) + odd), codes_h2(a0, 0x4140u), codes_h2(a0, 0x4342u), codes_h2(a1, 0x4140u), codes_h2(a1, 0x4342u));
+            sts128(swizzled(tile, r, (piece & 7) + 1 - odd), codes_h2(a2, 0x4140u), codes_h2(a2, 0x4342u), codes_h2(a3, 0x4140u), codes_h2(a3, 0x4342u));
           }
-          if (lane == 0) scale_s[warp] = make_float4(unit[0], log2_of(unit[1]), inverse_of(unit[1]), 0.f);
+          if (lane == 0) {
+            const float ks = there ? raw_scale_s[warp].x : 1.f, vs = there ? raw_scale_s[warp].y : 1.f;
+            scale_s[warp] = make_float4(ks, log2_of(vs), fminf(inverse_of(vs), 3.0e38f), 0.f);
+          }
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // generic writes -> the product's reads
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncthreads();
-        if (idle || pos0 > x.s.start + min(warp_last, x.s.n - 1)) continue;  // none of the warp's rows sees the unit
+        if (tid == 0) {
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            mma_f16(tmem_s, smem_desc_sw128(q_a + (k >> 2) * kManyTile * 128 + (k & 3) * 32),
+                    smem_desc_sw128(k_a + (k >> 2) * kManyUnit * 128 + (k & 3) * 32), many_idesc(kManyUnit), k > 0);
+          mma_commit(bar_scores);
+        }
 
-        // ---- scores of 16 rows and 64 tokens
-        float acc[NT][4];
+        // ---- values: fp16 tile [dim][token] of the output product. A thread takes a pair of tokens and a
+        // quarter of the dims.
+        if (u > ua && !mbar_wait(bar_outputs, phase ^ 1)) dead_s = 1;
+        {
+          constexpr int N = D / 4;  // dims
+          if (tail) {
+            const float vlift = lift_s[lane >> 3].y;
+#pragma unroll 1
+            for (int i = 0; i < N / 8; ++i) {
+              uint4 v[2];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+              for (int e = 0; e < 2; ++e) {
+                const int pos = pos0 + 2 * lane + e;
+                const int64_t at = (((int64_t)b * c.kv_heads + h) * 2 * P + (pos & (2 * P - 1))) * D + warp * N + i * 8;
+                v[e] = pos < L ? *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(c.v_ring) + at) : make_uint4(0u, 0u, 0u, 0u);
+              }
+              const uint32_t w0[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, w1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-          for (int j = 0; j < NT; j += 2) {
-            uint32_t w[4];
-            ldmatrix4(w, k_row + j * 8 * RB + (((2 * k + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
-            mma16(acc[j], qa[k][0], qa[k][1], qa[k][2], qa[k][3], w[0], w[1]);
-            mma16(acc[j + 1], qa[k][0], qa[k][1], qa[k][2], qa[k][3], w[2], w[3]);
-          }
-        const bool masked = pos0 + kRowsUnit - 1 > min(x.s.start + warp_first, end - 1);
-        float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const float4 sc = scale_s[j >> 1];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            acc[j][i] = fmaf(acc[j][i], qu[i >> 1] * sc.x, sc.y);
-            if (masked) {
-              const int pos = pos0 + j * 8 + q4 * 2 + (i & 1);
-              if (pos > seen[i >> 1] || pos >= end) acc[j][i] = -INFINITY;
+              for (int k = 0; k < 4; ++k) {
+                const float2 a = pair_of<T>(w0[k]), e = pair_of<T>(w1[k]);
+                const int d = warp * N + i * 8 + 2 * k;
+                sts32(swizzled(v_a, d, lane >> 2) + (lane & 3) * 4, as_u32(__floats2half2_rn(a.x * vlift, e.x * vlift)));
+                sts32(swizzled(v_a, d + 1, lane >> 2) + (lane & 3) * 4, as_u32(__floats2half2_rn(a.y * vlift, e.y * vlift)));
+              }
             }
-            mx[i >> 1] = fmaxf(mx[i >> 1], acc[j][i]);
-          }
-        }
-        if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f)) {
+          } else {
+            const bool there = pos0 + 2 * lane < code_end;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float to = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-            to = fmaxf(fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 2)), m[e]);
-            const float corr = exp2_of(m[e] - to);
-            m[e] = to;
-            l[e] *= corr;
+            for (int i = 0; i < N / 16; ++i) {
+              uint4 v[2];
 #pragma unroll
-            for (int i = 0; i < DT; ++i) {
-              o[i][2 * e] *= corr;
-              o[i][2 * e + 1] *= corr;
+              for (int e = 0; e < 2; ++e)
+                v[e] = there ? lds128m(raw_v + (2 * lane + e) * D + (((warp * (N / 16) + i) ^ (lane & (D / 16 - 1))) << 4)) : make_uint4(0u, 0u, 0u, 0u);
+              const uint32_t w0[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, w1[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t a = w0[k] ^ 0x80808080u, e = w1[k] ^ 0x80808080u;
+                const uint32_t lo = __byte_perm(a, e, 0x5140u), hi = __byte_perm(a, e, 0x7362u);
+                const int d = warp * N + i * 16 + 4 * k;
+                const uint32_t at = (lane & 3) * 4;
+                sts32(swizzled(v_a, d, lane >> 2) + at, codes_h2(lo, 0x4140u));
+                sts32(swizzled(v_a, d + 1, lane >> 2) + at, codes_h2(lo, 0x4342u));
+                sts32(swizzled(v_a, d + 2, lane >> 2) + at, codes_h2(hi, 0x4140u));
+                sts32(swizzled(v_a, d + 3, lane >> 2) + at, codes_h2(hi, 0x4342u));
+              }
             }
           }
         }
-        uint32_t pa[NT][2];
+
+        // ---- this thread's row of scores to weights
+        if (!mbar_wait(bar_scores, phase)) dead_s = 1;
+        __syncwarp();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const bool masked = pos0 + kManyUnit - 1 > min(x.s.start + x.t_lo, end - 1);
+        const int last = min(seen, end - 1) - pos0;  // of this unit's tokens, the last one the row sees
+        float s[kManyUnit], mx = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const float inv = scale_s[j >> 1].z;
+        for (int half = 0; half < 2; ++half) {
+          uint32_t w[32];
+          tmem_ld32(tmem + half * 32, w);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float w0 = exp2_of(acc[j][2 * e] - m[e]), w1 = exp2_of(acc[j][2 * e + 1] - m[e]);
-            l[e] = fmaf(w0 + w1, inv, l[e]);
-            pa[j][e] = as_u32(__floats2half2_rn(w0, w1));
+          for (int i = 0; i < 32; ++i) {
+            const float4 sc = scale_s[half * 2 + (i >> 4)];
+            float v = fmaf(__uint_as_float(w[i]), qu * sc.x, sc.y);
+            if (masked && half * 32 + i > last) v = -INFINITY;
+            s[half * 32 + i] = v;
+            mx = fmaxf(mx, v);
+          }
+        }
+        if (__any_sync(0xffffffffu, mx > m + 8.f)) {
+          const float to = fmaxf(m, mx), corr = exp2_of(m - to);
+          m = to;
+          l *= corr;
+          if (u > ua) {  // (the first unit's product writes the outputs afresh)
+#pragma unroll 1
+            for (int i = 0; i < D / 32; ++i) {
+              uint32_t w[32];
+              tmem_ld32(tmem + kOutCol + i * 32, w);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(__uint_as_float(w[k]) * corr);
+              tmem_st32(tmem + kOutCol + i * 32, w);
+            }
           }
         }
 #pragma unroll
-        for (int k = 0; k < NT / 2; ++k)
+        for (int e = 0; e < 4; ++e) {
+          float sum = 0.f;
+          uint32_t w[8];
 #pragma unroll
-          for (int d = 0; d < DT; d += 2) {
-            uint32_t w[4];
-            ldmatrix4_trans(w, v_row + k * 16 * RB + (((d + (lane >> 4)) ^ (lane & 7)) << 4));
-            mma16(o[d], pa[2 * k][0], pa[2 * k][1], pa[2 * k + 1][0], pa[2 * k + 1][1], w[0], w[1]);
-            mma16(o[d + 1], pa[2 * k][0], pa[2 * k][1], pa[2 * k + 1][0], pa[2 * k + 1][1], w[2], w[3]);
+          for (int i = 0; i < 8; ++i) {
+            const float w0 = exp2_of(s[e * 16 + 2 * i] - m), w1 = exp2_of(s[e * 16 + 2 * i + 1] - m);
+            sum += w0 + w1;
+            w[i] = as_u32(__floats2half2_rn(w0, w1));
           }
+          l = fmaf(sum, scale_s[e].z, l);
+          sts128(swizzled(p_a, tid, 2 * e), w[0], w[1], w[2], w[3]);
+          sts128(swizzled(p_a, tid, 2 * e + 1), w[4], w[5], w[6], w[7]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncthreads();
+        if (dead_s) break;
+        if (tid == 0) {
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_f16(tmem_s + kOutCol, smem_desc_sw128(p_a + k * 32), smem_desc_sw128(v_a + k * 32), many_idesc(D), u > ua || k > 0);
+          mma_commit(bar_outputs);
+        }
+        issue(u + 1);  // (every thread has read this unit's codes)
+        phase ^= 1;
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
+      if (dead_s || !mbar_wait(bar_outputs, phase ^ 1)) dead_s = 1;
+      __syncwarp();
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 
       // ---- what this run has of the (sequence, head): all of it, or a part
       const bool whole = ua == 0 && ub == x.units;
-      const int64_t slot = ((int64_t)rt * (gridDim.x + heads) + blockIdx.x + b * c.kv_heads + h) * kRowsTile;
-      if (threadIdx.x == 0) {  // for the join: the runs that begin and end it
+      const int64_t slot = ((int64_t)rt * (gridDim.x + heads) + blockIdx.x + b * c.kv_heads + h) * kManyTile;
+      if (tid == 0) {  // for the join: the runs that begin and end it
         if (ua == 0) ends[(int64_t)rt * heads + b * c.kv_heads + h].x = blockIdx.x;
         if (ub == x.units) ends[(int64_t)rt * heads + b * c.kv_heads + h].y = blockIdx.x;
       }
+      const float inv = live ? 1.f / l : 0.f;
+#pragma unroll 1
+      for (int i = 0; i < D / 32; ++i) {
+        uint32_t w[32];
+        tmem_ld32(tmem + kOutCol + i * 32, w);
+        if (row >= sh.rows) {
+        } else if (whole) {
+          uint4* dst = reinterpret_cast<uint4*>(out + (((int64_t)b * sp.tokens + tok) * sh.Hq + h * sh.G + g) * D + i * 32);
+          uint32_t y[16];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float sum = l[e];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        const int row = row0 + 8 * e, r = warp * 16 + gid + 8 * e, g = row - tok[e] * sh.G;
-        if (row >= sh.rows) continue;
-        if (whole) {
-          const bool live = tok[e] < x.s.n;
-          const float inv = live ? 1.f / sum : 0.f;
-          uint32_t* dst = reinterpret_cast<uint32_t*>(out + (((int64_t)b * sp.tokens + tok[e]) * sh.Hq + h * sh.G + g) * D) + q4;
+          for (int k = 0; k < 16; ++k)
+            y[k] = live ? pair_to<T>(__uint_as_float(w[2 * k]) * inv, __uint_as_float(w[2 * k + 1]) * inv) : 0u;
 #pragma unroll
-          for (int i = 0; i < DT; ++i) dst[4 * i] = live ? pair_to<T>(o[i][2 * e] * inv, o[i][2 * e + 1] * inv) : 0u;
+          for (int k = 0; k < 4; ++k) dst[k] = make_uint4(y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]);
         } else {
-          float2* dst = reinterpret_cast<float2*>(part + (slot + r) * D) + q4;
+          uint4* dst = reinterpret_cast<uint4*>(part + (slot + tid) * D + i * 32);
 #pragma unroll
-          for (int i = 0; i < DT; ++i) dst[4 * i] = make_float2(o[i][2 * e], o[i][2 * e + 1]);
-          if (q4 == 0) part_ml[slot + r] = make_float2(m[e], sum);
+          for (int k = 0; k < 8; ++k) dst[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
         }
+        __syncwarp();
       }
-      __syncthreads();  // the shared memory is free for the next (sequence, head)
+      if (!whole && row < sh.rows) part_ml[slot + tid] = make_float2(m, l);
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncthreads();  // shared and tensor memory are free for the next (sequence, head)
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (dead_s) left = 0;
     }
     off -= x.units * c.kv_heads;
   }
+  if (dead_s && tid == 0) atomicExch(error_word, LQ_BLOCK_WAIT);
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_s), "r"(kManyCols) : "memory");
 }
 
 // ---------------------------------------------------------------- join the parts
@@ -1040,7 +1117,7 @@ block_attn_join_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
   // (start and count are older than the kernel ahead, which has waited for their writer)
   const Tile x = tile_of(c, sp, sh, b, rt);
   const int r0 = blockIdx.y / cols * rows_each, rows = min(rows_each, min(sh.tile, sh.rows - rt * sh.tile) - r0);
-  const int items = rows * V, groups = max(1, (int)blockDim.x / items);
+  const int items = max(rows, 1) * V, groups = max(1, (int)blockDim.x / items);
   const int group = threadIdx.x / items, item = threadIdx.x - group * items, r = item / V, d = (item - r * V + blockIdx.y % cols * V) * 4;
   const int row = rt * sh.tile + r0 + r, t = token_of(sh, row), g = row - t * sh.G;
   uint2* dst = reinterpret_cast<uint2*>(out + (((int64_t)b * sp.tokens + t) * sh.Hq + h * sh.G + g) * D + d);
@@ -1113,7 +1190,7 @@ block_attn_join_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
 
 // ---------------------------------------------------------------- host
 #ifndef LQ_ALONE
-#define LQ_ALONE 16
+#define LQ_ALONE 80
 #endif
 constexpr int kAloneRows = LQ_ALONE;
 
@@ -1131,10 +1208,10 @@ Plan plan_of(const lq_block_kv& c, int Hq, int T_new) {
   // Up to 16 rows the codes' bytes decide, and warps that work alone stream them best; more rows share
   // the conversion of a unit.
   p.nt = p.sh.rows <= 8 ? 1 : p.sh.rows <= kAloneRows ? 2 : 0;
-  p.sh.tile = p.nt ? 8 * p.nt : kRowsTile;
+  p.sh.tile = p.nt ? 8 * p.nt : kManyTile;
   p.sh.unit_log2 = p.nt ? 5 : 6;
   p.tiles = (p.sh.rows + p.sh.tile - 1) / p.sh.tile;
-  const int at_once = sm_count() * (p.nt == 0 ? kRowsCtas : p.nt == 2 ? Cfg<128, 2>::kWarps : c.head_dim == 64 ? Cfg<64, 1>::kWarps : Cfg<128, 1>::kWarps);
+  const int at_once = sm_count() * (p.nt == 0 ? kManyCtas : p.nt == 2 ? Cfg<128, 2>::kWarps : c.head_dim == 64 ? Cfg<64, 1>::kWarps : Cfg<128, 1>::kWarps);
   p.sh.slots = at_once / p.tiles > 1 ? at_once / p.tiles : 2;
   p.sh.step = (uint32_t)(0x100000000ULL / p.sh.slots);
   p.sh.waves = p.tiles == 1 ? 2 : 1;
@@ -1190,9 +1267,9 @@ struct Main {
 };
 template <typename T, int D>
 struct Main<T, D, 0> {
-  static auto kernel() { return block_attn_rows_kernel<T, D>; }
-  static constexpr size_t kSmem = RowsCfg<D>::kTotal;
-  static constexpr int kThreads = 32 * kRowsWarps;
+  static auto kernel() { return block_attn_many_kernel<T, D>; }
+  static constexpr size_t kSmem = ManyCfg<D>::kTotal;
+  static constexpr int kThreads = kManyThreads;
 };
 
 template <typename T, int D, int NT>

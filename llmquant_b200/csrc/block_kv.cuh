@@ -26,7 +26,7 @@ struct SeqSpan {
   int start, n;
 };
 
-enum { LQ_BLOCK_BAD_PAGE = 1, LQ_BLOCK_BAD_POSITION = 2, LQ_BLOCK_BAD_ANGLE = 3 };
+enum { LQ_BLOCK_BAD_PAGE = 1, LQ_BLOCK_BAD_POSITION = 2, LQ_BLOCK_BAD_ANGLE = 3, LQ_BLOCK_WAIT = 4 };
 
 // (start, count) of sequence b. A span that leaves the table's positions is treated as no tokens;
 // `bad` tells. count is cut to [0, tokens].

@@ -245,9 +245,10 @@ class BlockKVStore:
         with torch.cuda.device(self.device):
             word = native.library().lq_block_kv_device_error()
         if word:
-            what = {1: "a page id outside the pool", 2: "tokens outside the table",
-                    3: "a position outside the angle tables"}.get(word, f"error word {word}")
-            raise RuntimeError(f"block-scaled KV cache: a kernel met {what} and skipped it")
+            what = {1: "met a page id outside the pool and skipped it", 2: "met tokens outside the table and skipped them",
+                    3: "met a position outside the angle tables", 4: "gave up a wait for the tensor cores",
+                    }.get(word, f"left error word {word}")
+            raise RuntimeError(f"block-scaled KV cache: a kernel {what}")
 
 
 class BlockKVLayer(CacheLayerMixin):
