@@ -304,7 +304,7 @@ int lq_attn_decode_kv_i8_static(const void* q, const int8_t* k_codes, const int8
  * Nothing advances by itself: all layers of a step pass the same start. A sequence whose tokens
  * leave the table, a page id outside the pool and a position outside the angle tables are
  * skipped (read as NaN) and recorded: lq_block_kv_device_error() returns and clears 2, 1 or 3
- * (0 = none; it synchronizes with the device). */
+ * (4: a bounded wait for the tensor cores ran out; 0 = none; it synchronizes with the device). */
 typedef struct lq_block_kv {
   int8_t* k_pages;        /* [num_pages, kv_heads, block, head_dim], 16-byte aligned */
   int8_t* v_pages;
@@ -355,7 +355,9 @@ int lq_block_kv_append_qkv(const lq_block_kv* cache, const void* qkv, int64_t st
                            const int64_t* count_dev, int pdl, void* stream);
 
 /* Attention of the newest T_new rows over the cache as it stands after their append: row t of
- * sequence b sees the positions 0 .. start + t. q [B, T_new, Hq, D] by element strides of
+ * sequence b sees the positions 0 .. start + t. A value that is not finite makes NaN of the outputs of
+ * the rows that see its block (or its row, while the block is incomplete); in one call the rows of a
+ * sequence before it may be affected too. q [B, T_new, Hq, D] by element strides of
  * (b, t, head), D contiguous, 16-byte aligned rows; out [B, T_new, Hq, D] contiguous, zeros for
  * rows behind count. dtype float16 or bfloat16, any Hq / Hkv. `scratch`
  * (lq_block_attn_scratch_bytes, 16-byte aligned, no initial contents) holds the partial results of

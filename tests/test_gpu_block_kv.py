@@ -322,10 +322,10 @@ def filled(batch, heads, dim, block, dtype, lengths, seed, kstd=1.0, vstd=1.0):
 
 
 # The kernel's arithmetic before the last rounding: the weights as fp16 (half a step 2^-11, of each
-# weight), scores in fp32 whose absolute error in the exponent is at most 2^-24 times the sum of
-# |q| |k| over head_dim (cut to ~2^-14 for |scores| up to 60 as drawn here), outputs summed in
-# fp32. An output is a weighted mean of values, so all of it is within (2^-11 + 2^-13) of the largest
-# value; the query rows and bf16 ring rows are exact in fp16 after the lift.
+# weight); one group of bf16 queries as 15-bit integers (2^-14 of the row's largest value, so a score is
+# off by at most 2^-14 max|q| sum|k| scaling, under 2^-14 here for all but the sharpest rows, and
+# rms far less); scores in fp32. An output is a weighted mean of values, so all of it is within
+# (2^-11 + 2^-13) of the largest value; query rows in fp16 and ring rows are exact after the lift.
 EXTRA = 2.0 ** -11 + 2.0 ** -13
 
 
@@ -356,7 +356,8 @@ def test_attend_one_token(dtype, dim, heads, group):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("block", [16, 32, 64, 128])
-@pytest.mark.parametrize("tokens,group", [(2, 4), (5, 8), (17, 3), (64, 2), (150, 1)])
+@pytest.mark.parametrize("tokens,group", [(2, 4), (3, 3), (4, 4), (5, 8), (17, 3), (64, 2), (150, 1), (80, 1), (81, 1),
+                                          (43, 3), (129, 2)])
 def test_attend_several_tokens(dtype, block, tokens, group):
     """Drafts and chunks: causal inside the call, counts that differ, sequences that begin empty."""
     dim, heads = (128, 2) if block != 16 else (64, 1)
@@ -378,22 +379,24 @@ def test_attend_long_context_and_single_run():
     check_attend(store, model, q, [n - 1 for n in lengths], [1] * 200)
 
 
-def test_attend_blocks_of_very_different_scale():
+@pytest.mark.parametrize("tokens", [1, 5, 60])  # each of the kernels: 2, 10 and 120 rows
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attend_blocks_of_very_different_scale(tokens, dtype):
     """Value scales far apart, blocks of zeros, keys that decide: the folded scale must cancel."""
     block = 16
-    store, model = filled(1, 1, 64, block, torch.bfloat16, [0], 81)
-    store = pool_store(1, 1, 64, 8, block, torch.bfloat16)
-    k, v = rand((1, 1, 125, 64), 82).cuda(), rand((1, 1, 125, 64), 83).cuda()
+    model = Model(1, 1, 64, block, dtype)
+    store = pool_store(1, 1, 64, 8, block, dtype)
+    k, v = rand((1, 1, 125, 64), 82, dtype).cuda(), rand((1, 1, 125, 64), 83, dtype).cuda()
     for i, s in enumerate((1e-6, 1e4, 0.0, 1.0, 3e-3, 100.0, 1e-2, 1.0)):
         v[:, :, i * 16:(i + 1) * 16] *= s
     model.put(0, k[0], v[0], 0)
     store.append(k, v, 0)
     for std in (0.1, 2.0, 12.0):
-        q = rand((1, 1, 2, 64), 84, std=std).cuda()
-        check_attend(store, model, q, [124], [1])
+        q = rand((1, tokens, 2, 64), 84, dtype, std=std).cuda()
+        check_attend(store, model, q, [125 - tokens], [tokens])
     v[:] = 0.0
     store.append(k, v, 0)
-    assert (store.attend(q, 124) == 0).all()
+    assert (store.attend(q, 125 - tokens) == 0).all()
 
 
 def test_attend_strides_scratch_out_and_scaling():
@@ -404,41 +407,62 @@ def test_attend_strides_scratch_out_and_scaling():
     scratch = torch.empty(store.scratch_bytes(8, 1), dtype=torch.uint8, device="cuda").fill_(255)
     again = store.attend(q, torch.tensor([129, 89]).cuda(), scaling=0.3, out=out, scratch=scratch)
     assert again is out and torch.equal(out, got)
-    wide = torch.zeros(2, 1, 8, 256, dtype=q.dtype, device="cuda")[..., 1:129]  # rows on odd elements
-    wide.copy_(q)
-    assert torch.equal(store.attend(wide, torch.tensor([129, 89]).cuda(), scaling=0.3), got)
+    for tokens in (1, 4, 30):  # rows on odd elements, each of the kernels
+        q = rand((2, tokens, 8, 128), 95).cuda()
+        wide = torch.zeros(2, tokens, 8, 256, dtype=q.dtype, device="cuda")[..., 1:129]
+        wide.copy_(q)
+        start = torch.tensor([130 - tokens, 90 - tokens]).cuda()
+        assert torch.equal(store.attend(wide, start), store.attend(q, start))
 
 
-def test_attend_values_that_are_not_finite():
+@pytest.mark.parametrize("tokens", [1, 6, 50])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attend_values_that_are_not_finite(tokens, dtype):
     """What a sequence does not hold must not reach it: rubbish behind its length, other sequences."""
     block = 16
-    store, model = filled(2, 1, 64, block, torch.float16, [40, 20], 101)
-    q = rand((2, 1, 2, 64), 104, torch.float16).cuda()
-    want = store.attend(q, torch.tensor([39, 19]).cuda())
-    k = rand((2, 1, 8, 64), 105, torch.float16).cuda()
-    k[:] = math.nan
-    store.append(k[:, :, :4], k[:, :, :4], torch.tensor([40, 20]).cuda())  # taken back by the next call's start
-    assert torch.equal(store.attend(q, torch.tensor([39, 19]).cuda()), want)
+    lengths = [tokens + 39, tokens + 19]
+    store, model = filled(2, 1, 64, block, dtype, [n + 33 for n in lengths], 101)
+    q = rand((2, tokens, 2, 64), 104, dtype).cuda()
+    start = torch.tensor([39, 19]).cuda()
+    store.append(rand((2, 1, tokens, 64), 107, dtype).cuda(), rand((2, 1, tokens, 64), 108, dtype).cuda(), start)
+    want = store.attend(q, start)
+    assert want.isfinite().all()
+    k = torch.full((2, 1, 4, 64), math.nan, dtype=dtype, device="cuda")
+    store.append(k, k, torch.tensor(lengths).cuda())  # taken back by the next call's start
+    assert torch.equal(store.attend(q, start), want)
     # one sequence with NaN in a complete block: its rows only
-    k = rand((2, 1, 16, 64), 106, torch.float16).cuda()
+    k = rand((2, 1, 16, 64), 106, dtype).cuda()
     k[0, 0, 0, 0] = math.nan
-    store.append(k, k, torch.tensor([32, 16]).cuda())
-    got = store.attend(q, torch.tensor([47, 31]).cuda())
+    store.append(k, k, torch.tensor([16, 0]).cuda())
+    got = store.attend(q, start)
     assert got[0].isnan().all() and got[1].isfinite().all()
-    q[1, 0, 1, 3] = math.nan
-    got = store.attend(q, torch.tensor([31, 31]).cuda())
-    assert got[0].isfinite().all() and got[1, 0, 0].isfinite().all() and got[1, 0, 1].isnan().all()
+    k = rand((2, 1, 16, 64), 109, dtype).cuda()
+    store.append(k, k, torch.tensor([16, 0]).cuda())
+    assert store.attend(q, start).isfinite().all()
+    # a NaN in a row that is still in the ring: that sequence only
+    k = rand((2, 1, 1, 64), 110, dtype).cuda()
+    k[1] = math.inf
+    store.append(k, k, torch.tensor([n - 1 for n in lengths]).cuda())
+    got = store.attend(q, start)
+    assert got[0].isfinite().all() and not got[1, -1].isfinite().any()
+    # and a query that is not finite: its own row only
+    q[0, tokens - 1, 1, 3] = math.nan
+    got = store.attend(q, start)
+    assert got[0, tokens - 1, 1].isnan().all() and got[0, tokens - 1, 0].isfinite().all()
+    assert got[0, : tokens - 1].isfinite().all()
 
 
-def test_bad_pages_and_spans_are_skipped_and_reported():
+@pytest.mark.parametrize("tokens", [1, 6, 50])
+def test_bad_pages_and_spans_are_skipped_and_reported(tokens):
     store, model = filled(2, 1, 64, 16, torch.bfloat16, [64, 64], 111)
-    q = rand((2, 1, 2, 64), 114).cuda()
-    want = store.attend(q, torch.tensor([63, 63]).cuda())
+    q = rand((2, tokens, 2, 64), 114).cuda()
+    last = 64 - tokens
+    want = store.attend(q, torch.tensor([last, last]).cuda())
     table = store.table.clone()
     for bad in (-1, store.k_pages.shape[0], 2 ** 31 - 1):
         store.table[0, 1] = bad
-        got = store.attend(q, torch.tensor([63, 63]).cuda())
-        assert got[0].isnan().all() and torch.equal(got[1], want[1])
+        got = store.attend(q, torch.tensor([last, last]).cuda())
+        assert got[0, max(0, 16 - last):].isnan().all() and torch.equal(got[1], want[1])  # (the rows that see block 1)
         with pytest.raises(RuntimeError, match="page id outside the pool"):
             store.check_device_errors()
         k, _ = store.read(64, 64)
@@ -460,10 +484,46 @@ def test_bad_pages_and_spans_are_skipped_and_reported():
         assert torch.equal(store.k_ring.view(torch.int16), ring)
         with pytest.raises(RuntimeError, match="outside the table"):
             store.check_device_errors()
-        got = store.attend(q, torch.tensor([start, 63]).cuda())
+        got = store.attend(q, torch.tensor([start, last]).cuda())
         assert (got[0] == 0).all() and torch.equal(got[1], want[1])
         with pytest.raises(RuntimeError, match="outside the table"):
             store.check_device_errors()
+
+
+def test_counts_that_are_nothing_or_too_much():
+    store, model = filled(3, 1, 64, 32, torch.bfloat16, [70, 70, 70], 151)
+    for tokens in (1, 7, 100):
+        q = rand((3, tokens, 2, 64), 152).cuda()
+        none = torch.tensor([0, -5, -2 ** 40]).cuda()
+        assert (store.attend(q, torch.tensor([0, 30, 69]).cuda(), none) == 0).all()
+        before = store.k_ring.clone()
+        row = rand((3, 1, tokens, 64), 153).cuda()
+        store.append(row, row, torch.tensor([0, 30, 69]).cuda(), none)
+        assert torch.equal(before.view(torch.int16), store.k_ring.view(torch.int16))
+    q = rand((3, 4, 2, 64), 154).cuda()
+    start = torch.tensor([66, 40, 33]).cuda()  # (the ring reaches back to 32)
+    assert torch.equal(store.attend(q, start, torch.tensor([4, 2 ** 40, 99]).cuda()), store.attend(q, start))
+    store.check_device_errors()
+
+
+def test_a_pool_whose_offsets_pass_31_bits():
+    """Pages behind 2^31 bytes of codes: append, read and both attentions."""
+    heads, dim, block = 8, 128, 128
+    pages = 2 ** 31 // (heads * dim * block) + 40
+    codes = [torch.empty(pages, heads, block, dim, dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.empty(pages, heads, device="cuda") for _ in range(2)]
+    rings = [torch.empty(1, heads, 2 * block, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    table = torch.arange(pages - 1, pages - 9, -1, dtype=torch.int32, device="cuda")[None].contiguous()
+    store = BlockKVStore(*codes, *scales, *rings, table)
+    small = BlockKVStore.allocate(1, heads, dim, 8 * block, block)
+    k, v = rand((1, heads, 1000, dim), 161).cuda(), rand((1, heads, 1000, dim), 162).cuda()
+    for s in (store, small):
+        s.append(k, v, 0)
+    assert all(torch.equal(a, b) for a, b in zip(store.read(1000, 1000), small.read(1000, 1000)))
+    for tokens in (1, 40):
+        q = rand((1, tokens, 4 * heads, dim), 163).cuda()
+        assert torch.equal(store.attend(q, 1000 - tokens), small.attend(q, 1000 - tokens))
+    store.check_device_errors()
 
 
 # ------------------------------------------------------------------------------- together
@@ -530,10 +590,11 @@ def test_decode_in_a_graph_and_on_another_stream():
     assert model.block == block
 
 
-def test_two_stores_on_two_streams_at_once():
-    stores = [filled(4, 2, 128, 64, torch.bfloat16, [900, 1, 333, 64], 130 + i) for i in range(2)]
-    q = rand((4, 1, 16, 128), 139).cuda()
-    start = torch.tensor([899, 0, 332, 63]).cuda()
+@pytest.mark.parametrize("tokens", [1, 2, 24])
+def test_two_stores_on_two_streams_at_once(tokens):
+    stores = [filled(4, 2, 128, 64, torch.bfloat16, [900, tokens, 333, 64], 130 + i) for i in range(2)]
+    q = rand((4, tokens, 16, 128), 139).cuda()
+    start = torch.tensor([900 - tokens, 0, 333 - tokens, 64 - tokens]).cuda()
     want = [s.attend(q, start) for s, _ in stores]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(2)]
