@@ -336,7 +336,7 @@ struct AppendArgs {
 // a later block of the same parity replaces; its CTA then writes that later block's rows too,
 // after its own reads.
 template <typename T, int D, bool JOINED>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 2)
 block_append_kernel(const lq_block_kv c, const BlockSpan sp, const AppendArgs<T> p, const Rope rp, int* error_word) {
   constexpr int LPR = D / 8;  // lanes that hold a row
   __shared__ float red[kThreads / 32];
@@ -428,6 +428,7 @@ block_append_kernel(const lq_block_kv c, const BlockSpan sp, const AppendArgs<T>
 
   const bool to_ring = j >= last - 1 && !(reads_ring && j != first && ((j ^ first) & 1) == 0);
   const int pieces = P * LPR;
+  const int64_t page = complete ? page_of(c, b, j) : 0;  // (on its way while the rows are)
   Pack8<T> val[kMaxVec];
   Largest<T> top;
   constexpr int kStep = kThreads / LPR;  // rows between two pieces of a thread
@@ -470,7 +471,6 @@ block_append_kernel(const lq_block_kv c, const BlockSpan sp, const AppendArgs<T>
   const bool finite = amax <= 3.402823466e38f;
   const float scale = finite ? scale_of(amax, 127.f) : __int_as_float(0x7fffffff);
   const float inv = finite ? __fdiv_rn(1.f, scale) : 0.f;
-  const int64_t page = page_of(c, b, j);
   if (page < 0) {
     if (tid == 0) atomicExch(error_word, LQ_BLOCK_BAD_PAGE);
   } else {
