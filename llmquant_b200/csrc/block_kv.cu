@@ -9,7 +9,7 @@ namespace lq {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxVec = 8;  // 8-value pieces a thread holds of one block: 128 * 128 / 8 / 256
+constexpr int kMostPieces = 8;  // of 8 values that a thread holds of one block: 128 * 128 / 8 / 256
 
 // 8 consecutive values as they lie in memory, moved as 16-byte words
 template <typename T>
@@ -335,8 +335,8 @@ struct AppendArgs {
 // their maximum and writes the codes. The block that the call begins in may read ring rows that
 // a later block of the same parity replaces; its CTA then writes that later block's rows too,
 // after its own reads.
-template <typename T, int D, bool JOINED>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 2)
+template <typename T, int D, bool JOINED, int kMaxVec>  // kMaxVec: pieces of 8 values a thread holds of a block
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : kMaxVec > 4 ? 4 : 5)
 block_append_kernel(const lq_block_kv c, const BlockSpan sp, const AppendArgs<T> p, const Rope rp, int* error_word) {
   constexpr int LPR = D / 8;  // lanes that hold a row
   __shared__ float red[kThreads / 32];
@@ -543,15 +543,15 @@ block_read_kernel(const lq_block_kv c, const BlockSpan sp, T* __restrict__ k_out
   const T* ring = reinterpret_cast<const T*>(is_v ? c.v_ring : c.k_ring) + bh * 2 * P * D;
   const float nan = __int_as_float(0x7fffffff);
   if (complete) {
-    uint2 raw[kMaxVec];
+    uint2 raw[kMostPieces];
 #pragma unroll
-    for (int v = 0; v < kMaxVec; ++v) {
+    for (int v = 0; v < kMostPieces; ++v) {
       const int idx = tid + v * kThreads;
       raw[v] = make_uint2(0u, 0u);
       if (idx < rows * LPR && codes != nullptr) raw[v] = *reinterpret_cast<const uint2*>(codes + (int64_t)idx * 8);
     }
 #pragma unroll
-    for (int v = 0; v < kMaxVec; ++v) {
+    for (int v = 0; v < kMostPieces; ++v) {
       const int idx = tid + v * kThreads;
       if (idx >= rows * LPR) break;
       const int8_t* q = reinterpret_cast<const int8_t*>(&raw[v]);
@@ -620,11 +620,19 @@ int append(const lq_block_kv& c, const BlockSpan& sp, AppendArgs<T>& p, const Ro
   LQ_REQUIRE(y <= 65535, LQ_ERR_ARG, "%s: too many heads or tokens for one launch", what);
   const dim3 grid((unsigned)touched, y, (unsigned)c.batch);
   const cudaStream_t s = (cudaStream_t)stream;
-  if (c.head_dim == 64)
-    return joined ? launch(block_append_kernel<T, 64, true>, grid, s, pdl, what, c, sp, p, rp, error_word)
-                  : launch(block_append_kernel<T, 64, false>, grid, s, pdl, what, c, sp, p, rp, error_word);
-  return joined ? launch(block_append_kernel<T, 128, true>, grid, s, pdl, what, c, sp, p, rp, error_word)
-                : launch(block_append_kernel<T, 128, false>, grid, s, pdl, what, c, sp, p, rp, error_word);
+  // blocks of up to 8192 values leave a thread 4 pieces, fewer registers and so more CTAs on an SM
+  // (whole prompts, blocks of 64 x 128 and their read: 89 us with four CTAs, 77 with five, 79 with six)
+  const bool few = c.block * c.head_dim <= 4 * 8 * kThreads;
+#define LQ_APPEND(DD, JJ)                                                                                    \
+  return few ? launch(block_append_kernel<T, DD, JJ, 4>, grid, s, pdl, what, c, sp, p, rp, error_word)           \
+             : launch(block_append_kernel<T, DD, JJ, kMostPieces>, grid, s, pdl, what, c, sp, p, rp, error_word)
+  if (c.head_dim == 64) {
+    if (joined) LQ_APPEND(64, true);
+    LQ_APPEND(64, false);
+  }
+  if (joined) LQ_APPEND(128, true);
+  LQ_APPEND(128, false);
+#undef LQ_APPEND
 }
 
 }  // namespace
