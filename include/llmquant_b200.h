@@ -358,7 +358,7 @@ int lq_block_kv_append_qkv(const lq_block_kv* cache, const void* qkv, int64_t st
  * sequence b sees the positions 0 .. start + t. A value that is not finite makes NaN of the outputs of
  * the rows that see its block (or its row, while the block is incomplete); in one call the rows of a
  * sequence before it may be affected too. q [B, T_new, Hq, D] by element strides of
- * (b, t, head), D contiguous, 16-byte aligned rows; out [B, T_new, Hq, D] contiguous, zeros for
+ * (b, t, head), D contiguous; out [B, T_new, Hq, D] contiguous and 16-byte aligned, zeros for
  * rows behind count. dtype float16 or bfloat16, any Hq / Hkv. `scratch`
  * (lq_block_attn_scratch_bytes, 16-byte aligned, no initial contents) holds the partial results of
  * context slices; calls that may overlap need one each. */

@@ -1322,6 +1322,7 @@ extern "C" int lq_block_attn(const lq_block_kv* cache, const void* q, const int6
   if (const int rc = check_attn(cache, Hq, T_new, what)) return rc;
   LQ_REQUIRE(q && q_strides && out && scratch, LQ_ERR_ARG, "%s: null tensor pointer", what);
   LQ_REQUIRE(((uintptr_t)scratch & 15) == 0, LQ_ERR_ARG, "%s: scratch must be 16-byte aligned", what);
+  LQ_REQUIRE(((uintptr_t)out & 15) == 0, LQ_ERR_ARG, "%s: out must be 16-byte aligned", what);
   const Plan p = plan_of(*cache, Hq, T_new);
   LQ_REQUIRE(scratch_bytes_given >= scratch_bytes(*cache, p), LQ_ERR_ARG, "%s: scratch of %lld bytes, %lld are needed", what,
              (long long)scratch_bytes_given, (long long)scratch_bytes(*cache, p));

@@ -38,7 +38,8 @@ class BlockKVStore:
     int64 [batch] / [1] on the device) and `count` new rows that count (None: all of them, or
     int64 [batch]). Nothing advances by itself. `start` and `count` tensors are read on the GPU: what
     is wrong in them (tokens beyond the table, page ids outside the pool) is skipped there and
-    raised by `check_device_errors`."""
+    raised by `check_device_errors`. Calls run on torch's current stream of the cache's device and
+    can be captured into CUDA graphs, once one call of the kind has run outside a capture. No gradients."""
 
     def __init__(self, k_pages, v_pages, k_scales, v_scales, k_ring, v_ring, table):
         tensors = dict(k_pages=k_pages, v_pages=v_pages, k_scales=k_scales, v_scales=v_scales, k_ring=k_ring,
@@ -143,8 +144,8 @@ class BlockKVStore:
                    q_out=None, pdl=True):
         """From the fused projection's rows qkv [batch, tokens, q heads + 2 kv heads, head_dim]: queries and
         keys normed (weights given) and turned by their positions' angles, keys and values stored,
-        queries returned as [batch, tokens, q heads, head_dim]. One launch; the same values as
-        `qk_norm_rope` followed by `append`."""
+        queries returned as [batch, tokens, q heads, head_dim] (`q_out`, which must not overlap qkv, or
+        new). One launch; the same values as `qk_norm_rope` followed by `append`."""
         if qkv.dim() != 4 or qkv.shape[2] <= 2 * self.heads:
             raise RuntimeError(f"qkv must be [batch, tokens, q heads + {2 * self.heads}, head_dim], got {tuple(qkv.shape)}")
         _, tokens, heads, _ = qkv.shape
@@ -240,8 +241,9 @@ class BlockKVStore:
         return k, v
 
     def check_device_errors(self):
-        """Raise if a call since the last check met a bad `start`, `count`, page id or position (reads a
-        device word, so it synchronizes)."""
+        """Raise if a call since the last check met a bad `start`, `count`, page id or position (waits
+        for the work of all streams)."""
+        torch.cuda.synchronize(self.device)  # (the word is read on the default stream)
         with torch.cuda.device(self.device):
             word = native.library().lq_block_kv_device_error()
         if word:

@@ -88,6 +88,11 @@ def _head_norms(attn, head_dim):
     return (*(w.detach().to(torch.bfloat16).contiguous() for w in weights), eps[0])
 
 
+def has_head_norms(model) -> bool:
+    """Whether the attention of a model that is served (`supports`) normalises queries and keys for each head."""
+    return getattr(model.model.layers[0].self_attn, "q_norm", None) is not None
+
+
 def supports(model) -> bool:
     """Whether `model` is a Llama-layout decoder fully on kernel-mode linears."""
     try:
@@ -145,8 +150,7 @@ class FusedLlamaDecoder:
         dev, bf16 = self.device, torch.bfloat16
         # tokens to a block of the block-scaled cache, None for the cache with a scale per token;
         # the kernel of the latter has no place for norms of q and k
-        normed = _head_norms(model.model.layers[0].self_attn, self.D) is not None
-        self.kv_block = kv_block or (64 if normed else None)
+        self.kv_block = kv_block or (64 if has_head_norms(model) else None)
         if self.kv_block and kv_bits != 8:
             raise ValueError("the block-scaled KV cache (and with it a model that normalises queries and keys for "
                              f"each head) holds 8 bits, got kv_bits={kv_bits}")

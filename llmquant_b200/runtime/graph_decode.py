@@ -40,6 +40,8 @@ def can_graph(model, cache_factory=None) -> bool:
         if bits is None:
             return False  # some other cache class: not one this library can capture
         block = getattr(cache, "block_tokens", None)
+        if bits != 8 and fused.has_head_norms(model):
+            return False  # such a model is decoded on the block-scaled cache, which holds 8 bits
     model.__dict__["_graph_kv_cache_bits"] = bits
     model.__dict__["_graph_kv_block_tokens"] = block
     return True

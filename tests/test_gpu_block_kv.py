@@ -646,3 +646,22 @@ def test_refusals():
                      store.v_ring, store.table)
     with pytest.raises(RuntimeError, match="one of"):
         BlockKVStore.allocate(1, 1, 64, 32, 48)
+
+
+def test_errors_of_another_stream_are_reported():
+    store, _ = filled(1, 1, 64, 16, torch.bfloat16, [64], 141)
+    k = rand((1, 1, 1, 64), 142).cuda()
+    late = torch.tensor([64], device="cuda")  # one token behind a cache of 64
+    assert store.capacity == 64
+    store.append(k, k, late - 1)
+    store.check_device_errors()
+    busy = torch.randn(4096, 4096, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(50):  # (the call is still waiting for these when the check is made)
+            busy = busy @ busy
+        store.append(k, k, late)
+    with pytest.raises(RuntimeError, match="outside the table"):
+        store.check_device_errors()
+    store.check_device_errors()

@@ -221,6 +221,7 @@ def test_entry_points_choose_the_block_cache():
                        FusedLlamaDecoder(normed, 2, 33, kv_block=64).generate(ids, 12))
     with pytest.raises(ValueError, match="holds 8 bits"):
         FusedLlamaDecoder(normed, 2, 33, kv_bits=4)
+    assert can_graph(normed, make_cache_factory(8)) and not can_graph(normed, make_cache_factory(4))
     normed.model.layers[0].self_attn.q_norm = torch.nn.Identity()
     assert not supports(normed)  # norms of another kind: not served rather than left out
     assert isinstance(BlockKVStore.allocate(1, 1, 64, 1), BlockKVStore)

@@ -23,8 +23,8 @@ def append(c, k=4096, tokens=1):
     native.call("lq_block_kv_append", c, k, k, strides, strides, tokens, 0, 0, 0, 0, 0, 0)
 
 
-def attend(c, q=4096, hq=8, tokens=1, scratch=4096, size=1 << 30, strides=(1024, 1024, 128)):
-    native.call("lq_block_attn", c, q, (ctypes.c_int64 * 3)(*strides), 4096, scratch, size, hq, tokens, 0, 0, 0, 0, 0.1, 0, 0)
+def attend(c, q=4096, hq=8, tokens=1, scratch=4096, size=1 << 30, strides=(1024, 1024, 128), out=4096):
+    native.call("lq_block_attn", c, q, (ctypes.c_int64 * 3)(*strides), out, scratch, size, hq, tokens, 0, 0, 0, 0, 0.1, 0, 0)
 
 
 @pytest.mark.parametrize("fields,match", [
@@ -57,6 +57,8 @@ def test_bad_arguments_are_refused():
         attend(cache(), size=64)
     with pytest.raises(RuntimeError, match="scratch must be 16-byte aligned"):
         attend(cache(), scratch=4100)
+    with pytest.raises(RuntimeError, match="out must be 16-byte aligned"):
+        attend(cache(), out=4098)
     with pytest.raises(RuntimeError, match="empty output"):
         native.call("lq_block_kv_read", cache(), 4096, 4096, 0, 0, 0, 0, 0, 1, 0, 0)
     qkv = [4096, 1536, 1536, 4096, 8, 1, 0, 0, 1e-6, 64, 64, 10, 128, 0, 0, 0, 0, 0, 0, 0]
