@@ -82,6 +82,28 @@ __device__ __forceinline__ float inverse_of(float x) {
   return y;
 }
 
+// Two fp32 values in a register pair, for the instructions that work on both
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+
 // ---------------------------------------------------------------- how the line of units is cut
 constexpr int kFirst = 80;  // per cent of a long line that the warps which run at once take
 
@@ -812,13 +834,18 @@ block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
       left -= ub - ua;
       const int last_code = min(ub, x.code_units);
 
-      // codes of this warp's 16 tokens of a unit; the values' pieces of a row permuted by its pair of tokens
-      auto issue = [&](int u) {
+      // Codes of this warp's 16 tokens of a unit, keys and values requested apart: a unit's keys while the
+      // unit before is still at its scores, its values once that one's are converted. The page id is
+      // requested one unit earlier than the codes.
+      auto look_up = [&](int u) {
+        const int pos = u * kManyUnit + warp * 16;
+        return u < last_code && pos < code_end ? table[pos >> shift] : 0;
+      };
+      auto issue = [&](int u, int id, auto values) {
         const int pos = u * kManyUnit + warp * 16;
         if (u < last_code && pos < code_end) {
-          const int id = table[pos >> shift];
           if (id < 0 || id >= c.num_pages) {
-            if (lane == 0) {
+            if (!values && lane == 0) {
               atomicExch(error_word, LQ_BLOCK_BAD_PAGE);
               raw_scale_s[warp] = make_float2(__int_as_float(0x7fffffff), __int_as_float(0x7fffffff));
             }
@@ -828,15 +855,21 @@ block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
               const int idx = i * 32 + lane, r = warp * 16 + idx / (D / 16), piece = idx % (D / 16);
-              cp_async16(raw_k + r * D + piece * 16, c.k_pages + at + idx * 16);
-              cp_async16(raw_v + r * D + ((piece ^ ((r >> 1) & (D / 16 - 1))) << 4), c.v_pages + at + idx * 16);
+              // (the values' pieces of a row are permuted by its pair of tokens)
+              if (values) cp_async16(raw_v + r * D + ((piece ^ ((r >> 1) & (D / 16 - 1))) << 4), c.v_pages + at + idx * 16);
+              else cp_async16(raw_k + r * D + piece * 16, c.k_pages + at + idx * 16);
             }
-            if (lane < 2) cp_async4(smem_u32(&raw_scale_s[warp]) + lane * 4, (lane ? c.v_scales : c.k_scales) + ph);
+            if (!values && lane < 2) cp_async4(smem_u32(&raw_scale_s[warp]) + lane * 4, (lane ? c.v_scales : c.k_scales) + ph);
           }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
-      issue(ua);
+      const std::false_type keys{};
+      const std::true_type values{};
+      int page = look_up(ua);
+      issue(ua, page, keys);
+      issue(ua, page, values);
+      page = look_up(ua + 1);
 
       // ---- this thread's query row to its row of the A tile, lifted by a power of two
       float qu;
@@ -866,7 +899,7 @@ block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
         const int pos0 = tail ? x.held + (u - x.code_units) * kManyUnit : u * kManyUnit, mine = pos0 + warp * 16;
         const int end = tail ? L : code_end;  // positions that exist
         // ---- keys: fp16 tile of the score product (its last reader, the unit before's product, has ended)
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        asm volatile("cp.async.wait_group 1;" ::: "memory");  // (the values may still be on their way)
         if (tail) {  // 16 rows of the ring to a warp: what lifts them
           const int pos = mine + (lane >> 1);
           const int64_t at = (((int64_t)b * c.kv_heads + h) * 2 * P + (pos & (2 * P - 1))) * D + (lane & 1) * (D / 2);
@@ -924,6 +957,9 @@ block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
             scale_s[warp] = make_float4(ks, log2_of(vs), fminf(inverse_of(vs), 3.0e38f), 0.f);
           }
         }
+        __syncwarp();  // (the warp has read its keys)
+        issue(u + 1, page, keys);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");  // this unit's values
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // generic writes -> the product's reads
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncthreads();
@@ -991,19 +1027,30 @@ block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const bool masked = pos0 + kManyUnit - 1 > min(x.s.start + x.t_lo, end - 1);
         const int last = min(seen, end - 1) - pos0;  // of this unit's tokens, the last one the row sees
-        float s[kManyUnit], mx = -INFINITY;
+        uint64_t s[kManyUnit / 2];  // pairs of scores
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           uint32_t w[32];
           tmem_ld32(tmem + half * 32, w);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float4 sc = scale_s[half * 2 + (i >> 4)];
-            float v = fmaf(__uint_as_float(w[i]), qu * sc.x, sc.y);
-            if (masked && half * 32 + i > last) v = -INFINITY;
-            s[half * 32 + i] = v;
-            mx = fmaxf(mx, v);
+          for (int i = 0; i < 16; ++i) {
+            const float4 sc = scale_s[half * 2 + (i >> 3)];
+            const float by = qu * sc.x;
+            s[half * 16 + i] = fma2(pack2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1])), pack2(by, by), pack2(sc.y, sc.y));
           }
+        }
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < kManyUnit / 2; ++i) {
+            const float2 v = unpack2(s[i]);
+            s[i] = pack2(2 * i > last ? -INFINITY : v.x, 2 * i + 1 > last ? -INFINITY : v.y);
+          }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kManyUnit / 2; ++i) {
+          const float2 v = unpack2(s[i]);
+          mx = fmaxf(mx, fmaxf(v.x, v.y));
         }
         if (__any_sync(0xffffffffu, mx > m + 8.f)) {
           const float to = fmaxf(m, mx), corr = exp2_of(m - to);
@@ -1020,17 +1067,20 @@ block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
             }
           }
         }
+        const uint64_t minus_m = pack2(-m, -m);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float sum = 0.f;
+          uint64_t sums = 0;
           uint32_t w[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float w0 = exp2_of(s[e * 16 + 2 * i] - m), w1 = exp2_of(s[e * 16 + 2 * i + 1] - m);
-            sum += w0 + w1;
+            const float2 v = unpack2(add2(s[e * 8 + i], minus_m));
+            const float w0 = exp2_of(v.x), w1 = exp2_of(v.y);
+            sums = add2(sums, pack2(w0, w1));
             w[i] = as_u32(__floats2half2_rn(w0, w1));
           }
-          l = fmaf(sum, scale_s[e].z, l);
+          const float2 sum = unpack2(sums);
+          l = fmaf(sum.x + sum.y, scale_s[e].z, l);
           sts128(swizzled(p_a, tid, 2 * e), w[0], w[1], w[2], w[3]);
           sts128(swizzled(p_a, tid, 2 * e + 1), w[4], w[5], w[6], w[7]);
         }
@@ -1045,7 +1095,8 @@ block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
             mma_f16(tmem_s + kOutCol, smem_desc_sw128(p_a + k * 32), smem_desc_sw128(v_a + k * 32), many_idesc(D), u > ua || k > 0);
           mma_commit(bar_outputs);
         }
-        issue(u + 1);  // (every thread has read this unit's codes)
+        issue(u + 1, page, values);  // (every thread has read this unit's)
+        page = look_up(u + 2);
         phase ^= 1;
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
