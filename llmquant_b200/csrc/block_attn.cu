@@ -105,7 +105,10 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 }
 
 // ---------------------------------------------------------------- how the line of units is cut
-constexpr int kFirst = 80;  // per cent of a long line that the warps which run at once take
+// Per cent of a long line that the warps which run at once take. 70 / 80 / 90: one context of 131072 tokens
+// 62.3 / 62.6 / 63.9 us, 64 ragged sequences 62.6 / 63.7 / 67.5, 32 ragged sequences with their
+// append 56.9 / 56.8 / 59.3.
+constexpr int kFirst = 80;
 
 struct Shape {
   int Hq, G, rows, tile;  // query rows per KV head: T_new * G; rows of one pass
@@ -254,7 +257,12 @@ __device__ __forceinline__ float largest_of(const uint32_t (&w)[N]) {
 }
 
 // ---------------------------------------------------------------- main kernel
-// grid (runs of the line, row tiles), one warp. T is the type of q, out and the ring.
+// grid (runs of the line, row tiles), one warp. T is the type of q, out and the ring. Bound by the
+// latencies of a warp's units (12 warps on an SM, 1.8 instructions a cycle), by about 8 us before the
+// first unit and in the join, and by SMs that stream at different speeds. One row each, 32 query heads
+// on 8, bf16, with the join: one context of 131000 tokens (268 MB) 64 us, 4.2 TB/s, 0.65 of a copy's
+// rate; 64 ragged contexts to 6000 with heads of 64 (299 MB) 68 us, 4.4 TB/s, 0.68. The same kernel
+// that only loads the codes takes 48 us instead of 53 for the long context, before the join.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32, (Cfg<D, NT>::kWarps))
 block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const T* __restrict__ q, int64_t qsb, int64_t qst,
@@ -266,7 +274,8 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
   extern __shared__ __align__(16) uint8_t ring[];
   // One group of bf16 queries meets the codes as 15-bit integers in two byte planes: the codes then need
   // no conversion. fp16 queries keep their 11 bits as fp16; with more groups the conversion is shared
-  // and the integer product's lower rate counts (chunk of 512: 278 us by integers, 242 by fp16).
+  // and the integer product's lower rate counts (512 rows of 32 heads on 3499 tokens, two groups: 278 us
+  // by integers, 242 by fp16).
   constexpr bool kInt = NT == 1 && std::is_same<T, __nv_bfloat16>::value;
   constexpr int kTop = kInt ? 13 : 10;  // exponent that a row's largest value is lifted to
 
@@ -738,7 +747,10 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
 // all 128 rows, the values' tile transposed on the way (both operands of a product run along k). The
 // outputs are only touched, by a warp for its 32 rows, when a row's maximum rises by 2^8. Two CTAs on an
 // SM: while one converts or exponentiates the other's products run. The weights, scales, masks and
-// parts are the ones of the kernel above. Bound by the instructions around the products, not by them.
+// parts are the ones of the kernel above. Bound by the instructions around the products and their
+// latencies (8 warps on an SM, 1.24 instructions a cycle, the tensor pipe busy 18 % of the time): 512 rows of
+// 32 heads on 8 after 3499 tokens, 31.5 GFLOP in 115 us with 14 us of join, 274 TFLOP/s. Two threads to
+// a row (16 warps on an SM) take 127 us: what is done once a unit and thread is done twice.
 constexpr int kManyTile = 128, kManyThreads = 128, kManyUnit = 64, kManyCtas = 2;  // CTAs on an SM
 constexpr uint32_t kManyCols = 256, kOutCol = 64;  // columns of tensor memory a CTA takes; where the outputs begin
 
