@@ -1,9 +1,8 @@
 """The block-scaled KV cache and the norm + rotation of queries and keys, on a B200, against plain
 implementations in 64 bits that are written here from the definitions.
 
-Tolerances. A result rounded once to its type is off by at most half a step relative to itself
-(bf16 2^-9 of the value's binade top, i.e. eps/2 = 2^-8 relative, fp16 2^-11, fp32 2^-24); what the kernels do
-before that rounding is fp32, whose own error is stated beside each bound. Codes and scales are
+Tolerances. A result rounded once to its type is off by at most half a step, eps / 2 relative to
+itself (bf16 2^-8, fp16 2^-11, fp32 2^-24); what the kernels do before that rounding is fp32, whose own error is stated beside each bound. Codes and scales are
 exact: the same IEEE division and rounding as the definition, on values that are exact in fp32."""
 
 import math
