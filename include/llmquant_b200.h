@@ -304,7 +304,8 @@ int lq_attn_decode_kv_i8_static(const void* q, const int8_t* k_codes, const int8
  * Nothing advances by itself: all layers of a step pass the same start. A sequence whose tokens
  * leave the table, a page id outside the pool and a position outside the angle tables are
  * skipped (read as NaN) and recorded: lq_block_kv_device_error() returns and clears 2, 1 or 3
- * (4: a bounded wait for the tensor cores ran out; 0 = none; it synchronizes with the device). */
+ * (4: a bounded wait for the tensor cores ran out, and the outputs that it served are NaN; 0 =
+ * none; it synchronizes with the device). */
 typedef struct lq_block_kv {
   int8_t* k_pages;        /* [num_pages, kv_heads, block, head_dim], 16-byte aligned */
   int8_t* v_pages;

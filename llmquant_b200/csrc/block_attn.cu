@@ -22,6 +22,7 @@
 #include <type_traits>
 
 #include "block_kv.cuh"
+#include "block_parts.cuh"
 #include "tcgen05.cuh"
 
 namespace lq {
@@ -701,7 +702,7 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
 
       // ---- what this run has of the (sequence, head): all of it, or a part
       const bool whole = ua == 0 && ub == x.units;
-      const int64_t slot = ((int64_t)rt * (gridDim.x + heads) + blockIdx.x + b * c.kv_heads + h) * ROWS;
+      const int64_t slot = part_slot(rt, gridDim.x, heads, blockIdx.x, b * c.kv_heads + h, ROWS);
       if (lane == 0) {  // for the join: the runs that begin and end it
         if (ua == 0) ends[(int64_t)rt * heads + b * c.kv_heads + h].x = blockIdx.x;
         if (ub == x.units) ends[(int64_t)rt * heads + b * c.kv_heads + h].y = blockIdx.x;
@@ -844,6 +845,10 @@ block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
       const int ub = min(x.units, ua + left);
       off += ub - ua;
       left -= ub - ua;
+      if (dead_s) {  // a wait ran out: what this CTA would have begun has no parts
+        if (tid == 0 && ua == 0) ends[(int64_t)rt * heads + b * c.kv_heads + h].x = -1;
+        continue;
+      }
       const int last_code = min(ub, x.code_units);
 
       // Codes of this warp's 16 tokens of a unit, keys and values requested apart: a unit's keys while the
@@ -905,8 +910,9 @@ block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
       }
       float m = kNone, l = 0.f;
 
+      int u = ua;
 #pragma unroll 1
-      for (int u = ua; u < ub; ++u) {
+      for (; u < ub; ++u) {
         const bool tail = u >= x.code_units;
         const int pos0 = tail ? x.held + (u - x.code_units) * kManyUnit : u * kManyUnit, mine = pos0 + warp * 16;
         const int end = tail ? L : code_end;  // positions that exist
@@ -1112,13 +1118,24 @@ block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
         phase ^= 1;
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
-      if (dead_s || !mbar_wait(bar_outputs, phase ^ 1)) dead_s = 1;
+      // After a wait that ran out the products may still be at work on this memory: each is waited for once
+      // more, and what there is of the row becomes NaN.
+      bool gave_up = u < ub;
+      if (gave_up) mbar_wait(bar_scores, phase);
+      if (!mbar_wait(bar_outputs, phase ^ 1)) {
+        gave_up = true;
+        mbar_wait(bar_outputs, phase ^ 1);
+      }
+      if (gave_up) {
+        dead_s = 1;
+        l = __int_as_float(0x7fffffff);
+      }
       __syncwarp();
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 
       // ---- what this run has of the (sequence, head): all of it, or a part
       const bool whole = ua == 0 && ub == x.units;
-      const int64_t slot = ((int64_t)rt * (gridDim.x + heads) + blockIdx.x + b * c.kv_heads + h) * kManyTile;
+      const int64_t slot = part_slot(rt, gridDim.x, heads, blockIdx.x, b * c.kv_heads + h, kManyTile);
       if (tid == 0) {  // for the join: the runs that begin and end it
         if (ua == 0) ends[(int64_t)rt * heads + b * c.kv_heads + h].x = blockIdx.x;
         if (ub == x.units) ends[(int64_t)rt * heads + b * c.kv_heads + h].y = blockIdx.x;
@@ -1148,7 +1165,6 @@ block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncthreads();  // shared and tensor memory are free for the next (sequence, head)
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (dead_s) left = 0;
     }
     off -= x.units * c.kv_heads;
   }
@@ -1188,9 +1204,15 @@ block_attn_join_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
     return;
   }
   const int2 end = __ldcg(ends + (int64_t)rt * heads + blockIdx.x);
-  const int parts = end.y - end.x + 1;
+  const int parts = parts_between(end.x, end.y, runs);
   if (parts == 1 || rows <= 0) return;  // one warp had all of it and wrote the output
-  const int64_t slot = ((int64_t)rt * (runs + heads) + blockIdx.x + end.x) * sh.tile + r0 + r;
+  const bool live = t < x.s.n;
+  if (parts == 0) {  // nobody took it: a wait ran out
+    const float nan = live ? __int_as_float(0x7fffffff) : 0.f;
+    if (group == 0) *dst = make_uint2(pair_to<T>(nan, nan), pair_to<T>(nan, nan));
+    return;
+  }
+  const int64_t slot = part_slot(rt, runs, heads, end.x, blockIdx.x, sh.tile) + r0 + r;
   const float2* ml = part_ml + slot;
   const float* mine = part + slot * D + d;
   float m = kNone, l = 0.f;
@@ -1243,7 +1265,6 @@ block_attn_join_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
     }
   }
   if (group != 0) return;
-  const bool live = t < x.s.n;
   const float inv = 1.f / l;
   *dst = live ? make_uint2(pair_to<T>(acc.x * inv, acc.y * inv), pair_to<T>(acc.z * inv, acc.w * inv)) : make_uint2(0u, 0u);
 }
