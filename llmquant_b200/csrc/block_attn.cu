@@ -352,7 +352,13 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
             copy(ids.x, pos & (P - 1), 0, stage, std::integral_constant<int, 2>());
           } else {
             copy(ids.x, 0, 0, stage, std::integral_constant<int, 1>());
-            if (pos + 16 < code_end) copy(ids.y, 0, 1, stage, std::integral_constant<int, 1>());
+            if (pos + 16 < code_end) {
+              copy(ids.y, 0, 1, stage, std::integral_constant<int, 1>());
+            } else if (lane < 2) {
+              // A unit's second half that is not there: its weights are 0, whatever the bytes of its codes, but
+              // 0 times the inverse of whatever its scales held before may be a NaN in the sum.
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(ring_a + stage * C::kStage + 2 * C::kCodes + 8 + lane * 4), "f"(1.f) : "memory");
+            }
           }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");

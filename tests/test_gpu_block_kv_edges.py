@@ -1,0 +1,36 @@
+"""The block-scaled KV cache at its edges, on a B200."""
+
+import pytest
+import torch
+
+from llmquant_b200.quantizers import BlockKVStore
+from test_gpu_block_kv import check_attend, filled, rand
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------- half a unit
+def leave_scales(dim, tokens, group, dtype, word):
+    """A call of the same kernel that leaves `word` where it stages scales, in every CTA that an SM holds: one
+    unit to a CTA, each the whole of its (sequence, head), so that no join runs over it."""
+    heads = 8
+    batch = 16 * torch.cuda.get_device_properties(0).multi_processor_count // heads
+    store = BlockKVStore.allocate(batch, heads, dim, 32, 32, dtype)
+    for scales in (store.k_scales, store.v_scales):
+        scales.view(torch.int32).fill_(word)
+    store.attend(rand((batch, tokens, heads * group, dim), 7, dtype).cuda(), 32 - tokens)
+
+
+@pytest.mark.parametrize("word", [-2 ** 31, -2 ** 31 + 1, -2 ** 31 + 0x7fffff, 0, 0x7f800000, 0x7fc00000, -1])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,tokens", [(64, 1), (64, 3), (128, 1), (128, 3)])  # 4 and 12 rows
+def test_an_odd_number_of_short_blocks_whatever_shared_memory_held(dim, tokens, dtype, word):
+    """Blocks of 16 are staged two to a unit: with three of them the last unit's second half is not there."""
+    store, model = filled(8, 2, dim, 16, dtype, [48] * 8, 201)
+    q = rand((8, tokens, 8, dim), 204, dtype, 2.0).cuda()
+    leave_scales(dim, tokens, 4, dtype, word)
+    check_attend(store, model, q, [48 - tokens] * 8, [tokens] * 8)
+    # and behind a whole unit, with rows of the incomplete block after it
+    store, model = filled(8, 2, dim, 16, dtype, [16 * 5 + 3] * 8, 205)
+    leave_scales(dim, tokens, 4, dtype, word)
+    check_attend(store, model, q, [83 - tokens] * 8, [tokens] * 8)
