@@ -75,6 +75,26 @@ def _unwrap(module):
     return getattr(module, "inner", module)
 
 
+@torch.no_grad()
+def _is_rms_norm(norm, weight, eps):
+    """Whether `norm` computes x * rsqrt(mean(x^2) + eps) * weight, seen on a few rows: neither its class nor
+    its attributes tell (others take the mean off, or scale by 1 + weight, and have the same ones)."""
+    rows = torch.randn(3, weight.shape[0], generator=torch.Generator().manual_seed(0)) + 1.0  # (with a mean)
+    rows[1] *= max(eps, 1e-12) ** 0.5  # eps counts here
+    rows[2] *= 16.0
+    x = rows.to(weight.device, weight.dtype)
+    try:
+        got = norm(x)
+    except (RuntimeError, TypeError, ValueError):
+        return False
+    if not isinstance(got, torch.Tensor) or got.shape != x.shape:
+        return False
+    want = x.double() * torch.rsqrt(x.double().square().mean(-1, keepdim=True) + eps) * weight.double()
+    # modules round to their dtype after the norm and after the weight, half a step each, of fp32 arithmetic
+    bound = 2 * torch.finfo(weight.dtype).eps + 1e-5
+    return bool(((got.double() - want).abs() <= bound * want.abs() + 1e-12).all())
+
+
 def _head_norms(attn, head_dim):
     """(q weight, k weight, eps) of an attention that normalises queries and keys for each head, None
     for one without such norms; ValueError for norms of another kind."""
@@ -85,6 +105,8 @@ def _head_norms(attn, head_dim):
     eps = [getattr(m, "variance_epsilon", getattr(m, "eps", None)) for m in (q, k)]
     if any(w is None or tuple(w.shape) != (head_dim,) for w in weights) or None in eps or eps[0] != eps[1]:
         raise ValueError("the norms of queries and keys are not RMS norms over head_dim")
+    if not all(_is_rms_norm(*norm) for norm in zip((q, k), weights, eps)):
+        raise ValueError("the norms of queries and keys do not compute x * rsqrt(mean(x^2) + eps) * weight")
     return (*(w.detach().to(torch.bfloat16).contiguous() for w in weights), eps[0])
 
 
