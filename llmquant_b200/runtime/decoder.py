@@ -110,6 +110,17 @@ def _head_norms(attn, head_dim):
     return (*(w.detach().to(torch.bfloat16).contiguous() for w in weights), eps[0])
 
 
+# What the attention of a served model is made of. Anything else that it holds (norms of another name or in
+# another place, sinks, gates) takes part in its arithmetic in a way that the decoder does not know.
+_ATTENTION_PARTS = {"q_proj", "k_proj", "v_proj", "o_proj", "q_norm", "k_norm", "rotary_emb"}
+
+
+def _plain_attention(attn) -> bool:
+    strange = [m for name, m in attn.named_children() if name not in _ATTENTION_PARTS and not isinstance(m, torch.nn.Dropout)]
+    own = [*attn.parameters(recurse=False), *attn.buffers(recurse=False)]
+    return not strange and not own
+
+
 def has_head_norms(model) -> bool:
     """Whether the attention of a model that is served (`supports`) normalises queries and keys for each head."""
     return getattr(model.model.layers[0].self_attn, "q_norm", None) is not None
@@ -131,7 +142,7 @@ def supports(model) -> bool:
             return False
         mods = [_unwrap(getattr(attn, n, None)) for n in names]
         mods += [_unwrap(getattr(mlp, n, None)) for n in ("gate_proj", "up_proj", "down_proj")]
-        if not all(isinstance(m, KernelQuantLinear) and m._stream for m in mods):
+        if not all(isinstance(m, KernelQuantLinear) and m._stream for m in mods) or not _plain_attention(attn):
             return False
     head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
     try:

@@ -1,4 +1,5 @@
-"""Which attentions the fused decoder takes: norms of queries and keys are recognised by what they compute."""
+"""Which attentions the fused decoder takes: norms of queries and keys are recognised by what they compute,
+and an attention with parts that the decoder does not know is left to its own module."""
 
 import pytest
 import torch
@@ -51,6 +52,7 @@ def test_rms_norms_are_taken(dtype, eps):
     attn = attention(*norms, dtype)
     q, k, got = decoder._head_norms(attn, DIM)
     assert got == eps and torch.equal(q, norms[0].weight.data.bfloat16()) and torch.equal(k, norms[1].weight.data.bfloat16())
+    assert decoder._plain_attention(attn)
     torch_norms = [torch.nn.RMSNorm(DIM, eps=eps) for _ in range(2)]
     assert decoder._head_norms(attention(*torch_norms, dtype), DIM)[2] == eps
 
@@ -71,8 +73,24 @@ def test_norms_of_another_kind_are_not(make, dtype):
 
 def test_none_missing_and_different_norms():
     attn = attention(None, None)
-    assert decoder._head_norms(attn, DIM) is None
+    assert decoder._head_norms(attn, DIM) is None and decoder._plain_attention(attn)
     for pair in ((LlamaRMSNorm(DIM), None), (LlamaRMSNorm(2 * DIM), LlamaRMSNorm(2 * DIM)),
                  (LlamaRMSNorm(DIM, eps=1e-5), LlamaRMSNorm(DIM, eps=1e-6)), (torch.nn.Identity(), torch.nn.Identity())):
         with pytest.raises(ValueError):
             decoder._head_norms(attention(*pair), DIM)
+
+
+def test_an_attention_with_other_parts_is_not_plain():
+    """Norms behind the rotation under names of their own, parameters (sinks), gates."""
+    attn = attention(None, None)
+    attn.query_layernorm, attn.key_layernorm = LlamaRMSNorm(DIM), LlamaRMSNorm(DIM)
+    assert not decoder._plain_attention(attn)
+    attn = attention(None, None)
+    attn.sinks = torch.nn.Parameter(torch.zeros(4))
+    assert not decoder._plain_attention(attn)
+    attn = attention(None, None)
+    attn.register_buffer("gate", torch.zeros(4))
+    assert not decoder._plain_attention(attn)
+    attn = attention(None, None)
+    attn.dropout, attn.rotary_emb = torch.nn.Dropout(0.1), torch.nn.Identity()
+    assert decoder._plain_attention(attn)
