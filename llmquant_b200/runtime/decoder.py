@@ -16,9 +16,11 @@ tail of the kernel before it. One step is captured into a CUDA graph and replaye
 the write cursor of the KV cache lives in device memory. Prefill runs through the
 transformers modules (eagerly, as in the reference) into the same integer cache.
 
-With `kv_block` the cache is the block-scaled one (`quantizers/block_kv.py`), and the attention block
-is three launches: norms of q and k, RoPE and append of the q|k|v row; attention; the join of its parts.
-That is also the route of models whose attention normalises queries and keys for each head.
+With `kv_block` (16, 32, 64 or 128) the cache is the block-scaled one (`quantizers/block_kv.py`), and the
+attention block is three launches: norms of q and k, RoPE and append of the q|k|v row; attention; the
+join of its parts. With 0 it is the cache with a scale per token; a model whose attention normalises
+queries and keys for each head then takes one launch more than others, which norms and turns q and
+k in place. None is 64 for such a model and 0 for any other.
 
 The arithmetic (bf16 roundings of RMSNorm, RoPE, SiLU*mul and the residual adds) follows
 transformers' Llama modules, so greedy tokens match the module-by-module path.
@@ -28,6 +30,7 @@ import torch
 
 from llmquant_b200 import native
 from llmquant_b200.core.scheme import QuantizationScheme
+from llmquant_b200.cuda.ops import qk_norm_rope
 from llmquant_b200.quantizers.block_kv import BlockKVCache
 from llmquant_b200.quantizers.kernel import KernelQuantLinear
 from llmquant_b200.quantizers.kv_cache import KernelQuantCache
@@ -181,11 +184,11 @@ class FusedLlamaDecoder:
         self.scaling = self.D ** -0.5
         self.vocab = cfg.vocab_size
         dev, bf16 = self.device, torch.bfloat16
-        # tokens to a block of the block-scaled cache, None for the cache with a scale per token;
-        # the kernel of the latter has no place for norms of q and k
-        self.kv_block = kv_block or (64 if has_head_norms(model) else None)
-        if self.kv_block and kv_bits != 8:
-            raise ValueError("the block-scaled KV cache (and with it a model that normalises queries and keys for "
+        # tokens to a block of the block-scaled cache, None for the cache with a scale per token
+        self.head_norms = has_head_norms(model)
+        self.kv_block = (64 if self.head_norms else None) if kv_block is None else kv_block or None
+        if (self.kv_block or self.head_norms) and kv_bits != 8:
+            raise ValueError("the block-scaled KV cache (and any cache of a model that normalises queries and keys for "
                              f"each head) holds 8 bits, got kv_bits={kv_bits}")
 
         self.layers = []
@@ -211,11 +214,14 @@ class FusedLlamaDecoder:
             cos, sin = model.model.rotary_emb(probe, positions)
         self.cos = cos[0].to(bf16).contiguous()
         self.sin = sin[0].to(bf16).contiguous()
-        if self.kv_block:  # fp32, one value per pair
+        if self.kv_block or self.head_norms:  # fp32, one value per pair
             with torch.no_grad():
                 cos, sin = model.model.rotary_emb(probe.float(), positions)
             self.cos_half = cos[0, :, : self.D // 2].float().contiguous()
             self.sin_half = sin[0, :, : self.D // 2].float().contiguous()
+        if self.head_norms and not self.kv_block:
+            # q and k are normed and turned before the attention kernel, whose own rotation turns by nothing
+            self.cos, self.sin = torch.ones_like(self.cos), torch.zeros_like(self.sin)
 
         B, H = self.B, self.hidden
         inter = self.layers[0]["down"].in_features
@@ -268,7 +274,7 @@ class FusedLlamaDecoder:
         self.graph = None
         separate_reduce = self.tp is not None and self.exchange is None
         per_linear = 3 if self.decode_gemm else 1  # the decode GEMM is planes, product, finish
-        per_attention = 3 if self.kv_block else 1
+        per_attention = 3 if self.kv_block else 2 if self.head_norms else 1
         self.launches_per_step = (len(self.layers) * (4 * per_linear + per_attention + (2 if separate_reduce else 0)) + per_linear
                                   + (2 if self._glue else 0))
         if not self.tp:
@@ -323,6 +329,11 @@ class FusedLlamaDecoder:
             store.attend(self.q_rot.view(heads), self.pos, scaling=self.scaling, out=self.attn.view(heads),
                          scratch=self.block_scratch, pdl=pdl)
             return
+        if self.head_norms:
+            q_weight, k_weight, eps = spec["head_norms"]
+            rows = self.qkv.view(self.B, 1, -1, self.D)
+            heads = rows[:, :, : self.Hq], rows[:, :, self.Hq : self.Hq + self.Hkv]
+            qk_norm_rope(*heads, self.cos_half, self.sin_half, self.pos, q_weight, k_weight, eps, out=heads)
         native.call("lq_attn_decode_fused", self.qkv.data_ptr(), self.cos.data_ptr(),
                     self.sin.data_ptr(), cache.k_codes.data_ptr(), cache.v_codes.data_ptr(),
                     cache.k_scales.data_ptr(), cache.v_scales.data_ptr(), self.attn.data_ptr(),

@@ -41,7 +41,7 @@ def can_graph(model, cache_factory=None) -> bool:
             return False  # some other cache class: not one this library can capture
         block = getattr(cache, "block_tokens", None)
         if bits != 8 and fused.has_head_norms(model):
-            return False  # such a model is decoded on the block-scaled cache, which holds 8 bits
+            return False  # such a model is decoded on caches of 8 bits
     model.__dict__["_graph_kv_cache_bits"] = bits
     model.__dict__["_graph_kv_block_tokens"] = block
     return True
@@ -127,7 +127,7 @@ def graphed_generate(model, input_ids, max_new_tokens: int, kv_cache_bits=None, 
     prompt = input_ids.shape[1]
     if kv_cache_bits:
         dec = fused.FusedLlamaDecoder(model, input_ids.shape[0], prompt + max_new_tokens + 1,
-                                      kv_bits=kv_cache_bits, kv_block=kv_block_tokens)
+                                      kv_bits=kv_cache_bits, kv_block=kv_block_tokens or 0)
         return dec.generate(input_ids, max_new_tokens)
     dec = GraphedDecoder(model, prompt, max_new_tokens, batch=input_ids.shape[0])
     nxt = dec.prefill(input_ids)
