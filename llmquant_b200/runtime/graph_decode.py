@@ -112,10 +112,12 @@ def graphed_generate(model, input_ids, max_new_tokens: int, kv_cache_bits=None, 
 
     `kv_cache_bits` selects the integer KV cache (fused decoder), with `kv_block_tokens` the
     block-scaled one; None means the cache the last `can_graph(model, cache_factory)` call was
-    asked about, bf16 KV if there was none."""
+    asked about, bf16 KV if there was none (ValueError for `kv_block_tokens` then)."""
     if kv_cache_bits is None:  # what can_graph was asked about
         kv_cache_bits = model.__dict__.get("_graph_kv_cache_bits")
-        kv_block_tokens = kv_block_tokens or model.__dict__.get("_graph_kv_block_tokens")
+        kv_block_tokens = kv_block_tokens if kv_block_tokens is not None else model.__dict__.get("_graph_kv_block_tokens")
+    if kv_block_tokens is not None and not kv_cache_bits:
+        raise ValueError(f"kv_block_tokens={kv_block_tokens} is for the 8-bit KV cache: give kv_cache_bits=8 with it")
     if kv_cache_bits:
         from llmquant_b200.quantizers.kv_cache import make_cache_factory
 
