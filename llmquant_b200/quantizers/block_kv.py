@@ -328,9 +328,10 @@ class BlockKVLayer(CacheLayerMixin):
         self.append(key_states, value_states)
         if not self.fused_read:
             return self.dequantized()
-        # stand-ins of the right shape, tagged so that int_kv_attention knows what it was given
+        # Stand-ins of the right shape, tagged so that int_kv_attention knows what it was given. Codes, not rows
+        # of the model's dtype: an attention function that takes them for keys and values fails on the type.
         shape = (self.batch, self.heads, self.length, self.head_dim)
-        k, v = (r[:, :, :1].expand(shape) for r in (self.store.k_ring, self.store.v_ring))
+        k, v = (p[:1, :, :1].expand(shape) for p in (self.store.k_pages, self.store.v_pages))
         k.lq_layer = v.lq_layer = self
         return k, v
 

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from llmquant_b200.quantizers import BlockKVStore
+from llmquant_b200.quantizers import BlockKVCache, BlockKVStore
 from test_gpu_block_kv import check_attend, filled, rand
 
 pytestmark = pytest.mark.gpu
@@ -34,3 +34,18 @@ def test_an_odd_number_of_short_blocks_whatever_shared_memory_held(dim, tokens, 
     store, model = filled(8, 2, dim, 16, dtype, [16 * 5 + 3] * 8, 205)
     leave_scales(dim, tokens, 4, dtype, word)
     check_attend(store, model, q, [83 - tokens] * 8, [tokens] * 8)
+
+
+# ------------------------------------------------------------------------------- behind transformers' Cache
+def test_stand_ins_of_a_fused_read_are_no_keys_and_values():
+    """An attention function other than the library's must fail on them instead of computing with them."""
+    cache = BlockKVCache(32, fused_read=True)
+    rows = rand((2, 3, 40, 64), 211).cuda()
+    k, v = cache.update(rows, rows, 0)
+    assert k.shape == v.shape == (2, 3, 40, 64) and k.lq_layer is v.lq_layer is cache.layers[0]
+    assert k.dtype == v.dtype == torch.int8
+    q = rand((2, 3, 1, 64), 212).cuda()
+    with pytest.raises(RuntimeError):
+        torch.nn.functional.scaled_dot_product_attention(q, k, v)
+    with pytest.raises(RuntimeError):
+        q @ k.transpose(2, 3)
