@@ -356,9 +356,9 @@ int lq_block_kv_append_qkv(const lq_block_kv* cache, const void* qkv, int64_t st
                            const int64_t* count_dev, int pdl, void* stream);
 
 /* Attention of the newest T_new rows over the cache as it stands after their append: row t of
- * sequence b sees the positions 0 .. start + t. A value that is not finite makes NaN of the outputs of
- * the rows that see its block (or its row, while the block is incomplete); in one call the rows of a
- * sequence before it may be affected too. q [B, T_new, Hq, D] by element strides of
+ * sequence b sees the positions 0 .. start + t. A key or value that is not finite makes NaN of the outputs
+ * of the rows that see a position of its block (or its own position, while the block is incomplete), and
+ * of no others. q [B, T_new, Hq, D] by element strides of
  * (b, t, head), D contiguous; out [B, T_new, Hq, D] contiguous and 16-byte aligned, zeros for
  * rows behind count. dtype float16 or bfloat16, any Hq / Hkv. `scratch`
  * (lq_block_attn_scratch_bytes, 16-byte aligned, no initial contents) holds the partial results of

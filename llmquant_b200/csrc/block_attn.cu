@@ -62,9 +62,11 @@ __device__ __forceinline__ float lift_of(float amax, int top, float& unit) {
   unit = __uint_as_float((unsigned)(127 + e - top) << 23);
   return __uint_as_float((unsigned)(127 - e + top) << 23);
 }
-__device__ __forceinline__ float finite_abs(float x) {
-  const float m = fabsf(x);
-  return m <= 3.402823466e38f ? m : 0.f;
+__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// Two halves, 0 in the place of one that is not finite
+__device__ __forceinline__ uint32_t finite_h2(uint32_t v) {
+  return v & __hle2_mask(__habs2(as_h2(v)), __floats2half2_rn(65504.f, 65504.f));
 }
 
 __device__ __forceinline__ float exp2_of(float x) {
@@ -391,7 +393,7 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         float unit;
-        const float lift = lift_of(finite_abs(amax), kTop, unit);
+        const float lift = lift_of(is_finite(amax) ? amax : 0.f, kTop, unit);
         // (integers cannot carry a NaN: a row that is not finite gets it with its unit)
         unit = amax <= 3.402823466e38f ? unit * qk_scale : __int_as_float(0x7fffffff);
 #pragma unroll
@@ -625,36 +627,50 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
         for (int nt = 0; nt < NT; ++nt) acc[0][nt][0] = acc[0][nt][1] = acc[0][nt][2] = acc[0][nt][3] = 0.f;
         uint4 kx[2][2 * J];
         float kmax = 0.f, vmax = 0.f;
-        auto largest = [](const uint4& v, float& top) {
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 p = pair_of<T>(w[i]);
-            top = fmaxf(top, fmaxf(finite_abs(p.x), finite_abs(p.y)));
-          }
-        };
+        // A token with a value that is not finite: its key becomes NaN, and so its score for the rows that see it; the
+        // value itself counts as 0, so that a row that does not see the token (weight 0) is as without it.
+        uint32_t strange = 0u;
         auto row_of = [&](const void* rows, int pos) {
           return reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(rows) + (bh + (pos & (2 * P - 1))) * D);
         };
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int pos = pos0 + gid + e * 8;
-          const uint4* row = row_of(c.k_ring, pos) + q4 * 2 * J;
-#pragma unroll
-          for (int i = 0; i < 2 * J; ++i) {
-            kx[e][i] = pos < L ? row[i] : make_uint4(0u, 0u, 0u, 0u);
-            largest(kx[e][i], kmax);
-          }
-        }
         // (the values are read twice, the second time from L1: once for their maximum, once to multiply)
         auto value_piece = [&](int e, int i) {
           const int pos = pos0 + q4 * 2 + (e & 1) + (e >> 1) * 8;
           return pos < L ? row_of(c.v_ring, pos)[gid * (DPT / 8) + i] : make_uint4(0u, 0u, 0u, 0u);
         };
+        constexpr int kAtOnce = D == 64 ? 2 : 4;  // (heads of 64 have 128 registers: all four at once cost 72 us instead
+        // of 68 on 64 ragged contexts to 6000)
+#pragma unroll kAtOnce
+        for (int e = 0; e < 4; ++e) {
+          uint32_t w[DPT / 2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+          for (int i = 0; i < DPT / 8; ++i) {
+            const uint4 v = value_piece(e, i);
+            w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+          }
+          const float top = largest_of<T>(w);
+          vmax = fmaxf(vmax, is_finite(top) ? top : 0.f);
+          strange |= (is_finite(top) ? 0u : 1u) << (q4 * 2 + (e & 1) + (e >> 1) * 8);
+        }
+        strange = __reduce_or_sync(0xffffffffu, strange);
 #pragma unroll
-          for (int i = 0; i < DPT / 8; ++i) largest(value_piece(e, i), vmax);
+        for (int e = 0; e < 2; ++e) {
+          const int pos = pos0 + gid + e * 8;
+          const uint4* row = row_of(c.k_ring, pos) + q4 * 2 * J;
+#pragma unroll
+          for (int i = 0; i < 2 * J; ++i) kx[e][i] = pos < L ? row[i] : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t w[8 * J];
+#pragma unroll
+          for (int i = 0; i < 2 * J; ++i) {
+            w[4 * i] = kx[e][i].x; w[4 * i + 1] = kx[e][i].y; w[4 * i + 2] = kx[e][i].z; w[4 * i + 3] = kx[e][i].w;
+          }
+          const float top = largest_of<T>(w);
+          kmax = fmaxf(kmax, is_finite(top) ? top : 0.f);
+          kx[e][0].x |= !is_finite(top) || (strange >> (gid + e * 8) & 1u) ? 0x7fff7fffu : 0u;
+        }
         float ks[1], vs[1];
         const float klift = lift_of(warp_max(kmax), 10, ks[0]);
         if (kInt) ks[0] *= 8.f;  // the fp16 queries are lifted 2^3 less than the integers
@@ -693,8 +709,8 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const uint4 v = value_piece(e, i);
-            y[e][0] = lifted(v.x, vlift); y[e][1] = lifted(v.y, vlift);
-            y[e][2] = lifted(v.z, vlift); y[e][3] = lifted(v.w, vlift);
+            y[e][0] = finite_h2(lifted(v.x, vlift)); y[e][1] = finite_h2(lifted(v.y, vlift));
+            y[e][2] = finite_h2(lifted(v.z, vlift)); y[e][3] = finite_h2(lifted(v.w, vlift));
           }
 #pragma unroll
           for (int d = 0; d < 4; ++d) {  // value tile 4 i + d: dims 2 d, 2 d + 1 of the eight
@@ -901,7 +917,7 @@ block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
         load_words(raw, reinterpret_cast<const uint16_t*>(q) + b * qsb + tok * qst + (int64_t)(h * sh.G + g) * qsh, live, q_vec);
         const float amax = largest_of<T>(raw);
         float unit;
-        const float lift = lift_of(finite_abs(amax), 10, unit);
+        const float lift = lift_of(is_finite(amax) ? amax : 0.f, 10, unit);
         qu = amax <= 3.402823466e38f ? unit * qk_scale : __int_as_float(0x7fffffff);
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
@@ -928,6 +944,7 @@ block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
           const int pos = mine + (lane >> 1);
           const int64_t at = (((int64_t)b * c.kv_heads + h) * 2 * P + (pos & (2 * P - 1))) * D + (lane & 1) * (D / 2);
           float top[2] = {0.f, 0.f};
+          bool strange = false;  // (as in the kernel above)
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv)
 #pragma unroll 2
@@ -935,14 +952,13 @@ block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
               const uint4 v = pos < L ? reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(kv ? c.v_ring : c.k_ring) + at)[i]
                                       : make_uint4(0u, 0u, 0u, 0u);
               const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float2 p = pair_of<T>(w[k]);
-                top[kv] = fmaxf(top[kv], fmaxf(finite_abs(p.x), finite_abs(p.y)));
-              }
+              const float m = largest_of<T>(w);
+              if (is_finite(m)) top[kv] = fmaxf(top[kv], m);
+              else strange = true;
             }
           float unit[2];
           const float klift = lift_of(warp_max(top[0]), 10, unit[0]), vlift = lift_of(warp_max(top[1]), 7, unit[1]);
+          strange = __shfl_xor_sync(0xffffffffu, (int)strange, 1) != 0 || strange;  // (two lanes have a row)
           if (lane == 0) {
             lift_s[warp] = make_float2(klift, vlift);
             scale_s[warp] = make_float4(unit[0], log2_of(unit[1]), inverse_of(unit[1]), 0.f);
@@ -955,7 +971,7 @@ block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const float2 p = pair_of<T>(w[k]);
-              z[k] = as_u32(__floats2half2_rn(p.x * klift, p.y * klift));
+              z[k] = strange ? 0x7fff7fffu : as_u32(__floats2half2_rn(p.x * klift, p.y * klift));
             }
             const int piece = (lane & 1) * (D / 16) + i;
             sts128(swizzled(k_a + (piece >> 3) * kManyUnit * 128, warp * 16 + (lane >> 1), piece & 7), z[0], z[1], z[2], z[3]);
@@ -1017,8 +1033,8 @@ block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
               for (int k = 0; k < 4; ++k) {
                 const float2 a = pair_of<T>(w0[k]), e = pair_of<T>(w1[k]);
                 const int d = warp * N + i * 8 + 2 * k;
-                sts32(swizzled(v_a, d, lane >> 2) + (lane & 3) * 4, as_u32(__floats2half2_rn(a.x * vlift, e.x * vlift)));
-                sts32(swizzled(v_a, d + 1, lane >> 2) + (lane & 3) * 4, as_u32(__floats2half2_rn(a.y * vlift, e.y * vlift)));
+                sts32(swizzled(v_a, d, lane >> 2) + (lane & 3) * 4, finite_h2(as_u32(__floats2half2_rn(a.x * vlift, e.x * vlift))));
+                sts32(swizzled(v_a, d + 1, lane >> 2) + (lane & 3) * 4, finite_h2(as_u32(__floats2half2_rn(a.y * vlift, e.y * vlift))));
               }
             }
           } else {

@@ -1,10 +1,13 @@
 """The block-scaled KV cache at its edges, on a B200."""
 
+import math
+
 import pytest
 import torch
 
+from llmquant_b200 import native
 from llmquant_b200.quantizers import BlockKVCache, BlockKVStore
-from test_gpu_block_kv import check_attend, filled, rand
+from test_gpu_block_kv import EXTRA, attend64, check_attend, close_to, filled, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +52,31 @@ def test_stand_ins_of_a_fused_read_are_no_keys_and_values():
         torch.nn.functional.scaled_dot_product_attention(q, k, v)
     with pytest.raises(RuntimeError):
         q @ k.transpose(2, 3)
+
+
+# ------------------------------------------------------------------------------- values that are not finite
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("where", ["k", "v"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,tokens,group", [(64, 4, 2), (128, 6, 4), (64, 7, 9), (128, 70, 2)])  # 8, 24, 63, 140 rows
+def test_a_value_that_is_not_finite_reaches_the_rows_that_see_it(dim, tokens, group, dtype, where, bad):
+    """One value of one row: NaN for the rows that see a position of its block, or its own position while the
+    block is incomplete; the definition's values, without it, for the rows before."""
+    block, start = 32, 40
+    total = start + tokens
+    held = total - total % block
+    store, model = filled(1, 2, dim, block, dtype, [total], 221)
+    q = rand((1, tokens, 2 * group, dim), 224, dtype, 2.0).cuda()
+    want = attend64(q[0], *(model.values(rows[0]) for rows in (model.k, model.v)), start, dim ** -0.5)
+    largest = model.v[0].double().abs().max()
+    for at in sorted({start, start + 1, held - 1, held, total - 2, total - 1} & set(range(start, total))):
+        k, v = model.k[0].clone(), model.v[0].clone()
+        (k if where == "k" else v)[0, at, dim - 3] = bad
+        store.append(k[None].cuda(), v[None].cuda(), 0)
+        got = store.attend(q, start)[0]
+        first = max(0, (at if at >= held else at - at % block) - start)  # the first row that sees it
+        assert got[first:, :group].isnan().all(), at
+        if first:
+            close_to(got[:first, :group], want[:first, :group], dtype, EXTRA, largest)
+        close_to(got[:, group:], want[:, group:], dtype, EXTRA, largest)  # the other head
+    assert native.library().lq_block_kv_device_error() == 0
