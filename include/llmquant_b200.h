@@ -301,11 +301,14 @@ int lq_attn_decode_kv_i8_static(const void* q, const int8_t* k_codes, const int8
  * Every call is about `T_new` rows per sequence on top of `start` cached tokens: sequence b
  * starts at start_dev[b * start_stride] (start_stride 0 = one value for all) or, with start_dev
  * NULL, at `start`; the first count_dev[b] of its rows count (cut to [0, T_new]; NULL = all).
- * Nothing advances by itself: all layers of a step pass the same start. A sequence whose tokens
- * leave the table, a page id outside the pool and a position outside the angle tables are
- * skipped (read as NaN) and recorded: lq_block_kv_device_error() returns and clears 2, 1 or 3
- * (4: a bounded wait for the tensor cores ran out, and the outputs that it served are NaN; 0 =
- * none; it synchronizes with the device). */
+ * Nothing advances by itself: all layers of a step pass the same start. What is wrong in device
+ * words is skipped and recorded; lq_block_kv_device_error() returns and clears the last one:
+ *   1  a page id outside the pool: its block is not stored, and reads as NaN
+ *   2  a sequence whose tokens leave the table (start < 0 too): it has no tokens in this call;
+ *      nothing is stored, what is read back and the outputs of attention are zeros
+ *   3  a position outside the angle tables: the heads are NaN
+ *   4  a bounded wait for the tensor cores ran out: the outputs that it served are NaN
+ * (0 = none, -1 = it cannot be read; it synchronizes with the device). */
 typedef struct lq_block_kv {
   int8_t* k_pages;        /* [num_pages, kv_heads, block, head_dim], 16-byte aligned */
   int8_t* v_pages;
