@@ -4,7 +4,7 @@
 //
 // One pass over the cache. The codes go to the tensor cores as fp16 integers (exact); the scales
 // never touch an element: with key scale ks and value scale vs of a block,
-//   x_p = log2(e) scaling ks (q . code_p) + log2(vs),  M = running maximum of x,
+//   x_p = log2(e) scaling ks (q . code_p) + log2(vs),  M = a little below the running maximum of x,
 //   w_p = 2^(x_p - M)  (the weight with the value scale folded in),
 //   O  += w_p code_p,  sum += (sum of the block's w_p) / vs,   out = O / sum.
 //
@@ -30,6 +30,12 @@ namespace {
 
 constexpr int kUnit = 32;  // tokens, as two halves of 16 (the height of an MMA tile)
 constexpr float kNone = -1e30f;  // a maximum of nothing: below any score, and 2^(kNone - M) is zero
+// Weights are held as fp16, which keeps 11 bits from 2^-14 to 2^15: M is set 2^kUp below the maximum and
+// follows it when a weight would pass 2^kMost, so that what lies 2^-21 below the largest still has its bits.
+// Long contexts have many such: with M at the maximum, 131071 weights of 1.25 * 2^-24 of the largest, 1 % of
+// the sum, were off by a fifth.
+constexpr float kUp = 7.f, kMost = 15.f;
+constexpr int kLowestValue = -95;  // exponent below which ring values are lifted no further
 
 __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                       uint32_t b1) {
@@ -56,9 +62,9 @@ __device__ __forceinline__ uint32_t codes_h2(uint32_t biased, uint32_t sel) {
 
 // 2^e with e the exponent of the largest finite |x| (0 for none), as the power of two that brings
 // it to [2^top, 2^(top + 1)), and its reciprocal.
-__device__ __forceinline__ float lift_of(float amax, int top, float& unit) {
+__device__ __forceinline__ float lift_of(float amax, int top, float& unit, int lowest = -100) {
   int e = (int)(__float_as_uint(amax) >> 23) - 127;
-  e = amax > 0.f ? max(e, -100) : top;
+  e = amax > 0.f ? max(e, lowest) : top;
   unit = __uint_as_float((unsigned)(127 + e - top) << 23);
   return __uint_as_float((unsigned)(127 - e + top) << 23);
 }
@@ -467,10 +473,8 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
           for (int i = 0; i < 2; ++i) {
             mx[nt][i] = fmaxf(acc[0][nt][i], acc[0][nt][i + 2]);
             if (H == 2) mx[nt][i] = fmaxf(mx[nt][i], fmaxf(acc[H - 1][nt][i], acc[H - 1][nt][i + 2]));
-            rises = rises || mx[nt][i] > m[nt][i] + 8.f;
+            rises = rises || mx[nt][i] > m[nt][i] + kMost;
           }
-        // M follows the maximum only when a weight would pass 2^8: any M serves, and fp16 keeps 11
-        // bits of a weight up to 2^15
         if (__any_sync(0xffffffffu, rises)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -479,7 +483,7 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
               float to = fmaxf(mx[nt][i], __shfl_xor_sync(0xffffffffu, mx[nt][i], 4));
               to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 8));
               to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 16));
-              to = fmaxf(to, m[nt][i]);
+              to = fmaxf(to - kUp, m[nt][i]);
               const float corr = exp2_of(m[nt][i] - to);
               m[nt][i] = to;
               l[nt][i] *= corr;
@@ -674,7 +678,8 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
         float ks[1], vs[1];
         const float klift = lift_of(warp_max(kmax), 10, ks[0]);
         if (kInt) ks[0] *= 8.f;  // the fp16 queries are lifted 2^3 less than the integers
-        const float vlift = lift_of(warp_max(vmax), 7, vs[0]);
+        // (1 / vs up to 2^102, a weight up to 2^15, fewer than 2^7 rows: the sum stays finite)
+        const float vlift = lift_of(warp_max(vmax), 7, vs[0], kLowestValue);
         auto lifted = [](uint32_t v, float lift) {
           const float2 p = pair_of<T>(v);
           return as_u32(__floats2half2_rn(p.x * lift, p.y * lift));
@@ -768,7 +773,7 @@ block_attn_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, const
 // [128, D]; a thread reads its row of scores, so that maximum and sum need no exchange, and writes its
 // row of weights as the next product's A operand. The codes become fp16 tiles in shared memory once for
 // all 128 rows, the values' tile transposed on the way (both operands of a product run along k). The
-// outputs are only touched, by a warp for its 32 rows, when a row's maximum rises by 2^8. Two CTAs on an
+// outputs are only touched, by a warp for its 32 rows, when a row's maximum rises by 2^8 above the last one. Two CTAs on an
 // SM: while one converts or exponentiates the other's products run. The weights, scales, masks and
 // parts are the ones of the kernel above. Bound by the instructions around the products and their
 // latencies (8 warps on an SM, 1.24 instructions a cycle, the tensor pipe busy 18 % of the time): 512 rows of
@@ -957,7 +962,7 @@ block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
               else strange = true;
             }
           float unit[2];
-          const float klift = lift_of(warp_max(top[0]), 10, unit[0]), vlift = lift_of(warp_max(top[1]), 7, unit[1]);
+          const float klift = lift_of(warp_max(top[0]), 10, unit[0]), vlift = lift_of(warp_max(top[1]), 7, unit[1], kLowestValue);
           strange = __shfl_xor_sync(0xffffffffu, (int)strange, 1) != 0 || strange;  // (two lanes have a row)
           if (lane == 0) {
             lift_s[warp] = make_float2(klift, vlift);
@@ -1092,8 +1097,8 @@ block_attn_many_kernel(const lq_block_kv c, const BlockSpan sp, const Shape sh, 
           const float2 v = unpack2(s[i]);
           mx = fmaxf(mx, fmaxf(v.x, v.y));
         }
-        if (__any_sync(0xffffffffu, mx > m + 8.f)) {
-          const float to = fmaxf(m, mx), corr = exp2_of(m - to);
+        if (__any_sync(0xffffffffu, mx > m + kMost)) {
+          const float to = fmaxf(m, mx - kUp), corr = exp2_of(m - to);
           m = to;
           l *= corr;
           if (u > ua) {  // (the first unit's product writes the outputs afresh)

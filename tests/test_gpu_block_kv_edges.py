@@ -80,3 +80,30 @@ def test_a_value_that_is_not_finite_reaches_the_rows_that_see_it(dim, tokens, gr
             close_to(got[:first, :group], want[:first, :group], dtype, EXTRA, largest)
         close_to(got[:, group:], want[:, group:], dtype, EXTRA, largest)  # the other head
     assert native.library().lq_block_kv_device_error() == 0
+
+
+# ------------------------------------------------------------------------------- long contexts
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens,group", [(1, 2), (6, 2), (70, 2)])  # each of the kernels: 2, 12 and 140 rows
+def test_many_small_weights_beside_a_large_one(tokens, group, dtype):
+    """One token with nearly all of the weight and 131071 with 1.25 * 2^-24 of it each: together they count 1 %. So
+    many sequences share the pages that a warp (CTA) has a context to itself."""
+    heads, dim, block, length = 8, 64, 128, 131072
+    batch = 16 * torch.cuda.get_device_properties(0).multi_processor_count // heads
+    one = BlockKVStore.allocate(1, heads, dim, length, block, dtype)
+    one.k_scales.fill_(1.0)
+    one.v_scales.fill_(1.0 / 127.0)
+    one.v_pages.fill_(127)
+    one.v_pages[0, :, 0] = 0
+    one.k_pages[0, :, 0, 0] = 1
+    rings = [r.expand(batch, *r.shape[1:]).contiguous() for r in (one.k_ring, one.v_ring)]
+    store = BlockKVStore(one.k_pages, one.v_pages, one.k_scales, one.v_scales, *rings, one.table.expand(batch, -1).contiguous())
+    q = torch.zeros(batch, tokens, heads * group, dim, dtype=dtype, device="cuda")
+    q[..., 0] = 16.0
+    got = store.attend(q, length - tokens, scaling=math.log(2.0 ** 24 / 1.25) / 16)
+    rest = torch.arange(length - tokens, length, dtype=torch.float64) * 1.25 * 2.0 ** -24
+    want = (rest / (1 + rest))[None, :, None, None].expand(got.shape)
+    # a weight is held as fp16 up to 2^7 above the point that it is counted from, so what lies below 2^-21 of the
+    # largest is off by at most 2^-32 of it: 2^-15 in all. Exponents in fp32: 24 * 2^-24 of each weight.
+    close_to(got, want, dtype, 2.0 ** -15 + 2.0 ** -17, torch.tensor(1.0))
+    assert native.library().lq_block_kv_device_error() == 0
