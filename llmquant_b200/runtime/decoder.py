@@ -23,7 +23,10 @@ queries and keys for each head then takes one launch more than others, which nor
 k in place. None is 64 for such a model and 0 for any other.
 
 The arithmetic (bf16 roundings of RMSNorm, RoPE, SiLU*mul and the residual adds) follows
-transformers' Llama modules, so greedy tokens match the module-by-module path.
+transformers' Llama modules, so greedy tokens match the module-by-module path. On the block-scaled cache,
+and where queries and keys are normed, they are turned by angles in fp32 and rounded once, where the
+modules round after the norm, after its weight and in the rotation: closer to the formula, not bit for
+bit theirs.
 """
 
 import torch
@@ -552,8 +555,8 @@ class FusedLlamaDecoder:
         the last check cannot be trusted. Reads device words, so it synchronizes."""
         lib = native.library()
         words = {"gemv": lib.lq_gemv_device_error(), "attention": lib.lq_attn_device_error()}
-        if self.kv_block:
-            words["block cache"] = lib.lq_block_kv_device_error()
+        if self.kv_block or self.head_norms:
+            words["block cache, head norms"] = lib.lq_block_kv_device_error()
         if self.workspace is not None:
             words["decode gemm"] = lib.lq_decode_gemm_device_error()
         if self.tp:

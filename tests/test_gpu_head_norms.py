@@ -97,3 +97,18 @@ def test_norms_of_another_kind_and_strange_parts_are_not_served():
     assert supports(model)
     attn.query_layernorm = torch.nn.LayerNorm(64).to("cuda", torch.bfloat16)
     assert not supports(model)
+
+
+@pytest.mark.parametrize("block", [0, 64])
+def test_a_position_without_angles_is_reported(block):
+    """A decoder stepped behind its last position: heads without angles, said by the check after the step."""
+    model = _tiny(True, head_dim=64)
+    dec = FusedLlamaDecoder(model, 1, 64, use_graph=False, kv_block=block)
+    dec.start_empty(ids_of(1, 1)[:, 0])
+    dec.step()
+    dec.check_device_errors()
+    dec.cos_half, dec.sin_half = dec.cos_half[:1].contiguous(), dec.sin_half[:1].contiguous()
+    dec.step()  # position 1
+    with pytest.raises(RuntimeError, match="head norms"):
+        dec.check_device_errors()
+    dec.check_device_errors()
