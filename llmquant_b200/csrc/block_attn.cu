@@ -1338,7 +1338,8 @@ int check_attn(const lq_block_kv* c, int Hq, int T_new, const char* what) {
              "%s: %d query heads do not share %d KV heads evenly, or there are no rows", what, Hq, c->kv_heads);
   LQ_REQUIRE(c->dtype != LQ_F32, LQ_ERR_UNSUPPORTED, "%s: built for float16 and bfloat16 rows", what);
   const int64_t group = Hq / c->kv_heads, rows = T_new * group;
-  LQ_REQUIRE(c->kv_heads <= 65535 && rows <= 65535LL * 8 && (rows + 64) * group < 0x100000000LL, LQ_ERR_ARG,
+  // (token_of() is exact for row * group below 2^32, the rows that fill the last tile among them)
+  LQ_REQUIRE(c->kv_heads <= 65535 && rows <= 65535LL * 8 && (rows + kManyTile) * group < 0x100000000LL, LQ_ERR_ARG,
              "%s: too many rows for one call", what);
   LQ_REQUIRE((int64_t)c->batch * c->kv_heads * ((int64_t)c->max_blocks * c->block / kUnit + 2) < 0x7fffffffLL, LQ_ERR_ARG,
              "%s: batch, heads and positions together are too many for one call", what);

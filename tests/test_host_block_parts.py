@@ -55,3 +55,15 @@ def test_parts_of_one_tile_do_not_overlap(parts):
     line = [(0, 0), (0, 1), (1, 1), (2, 1), (2, 2), (2, 3), (3, 4), (4, 4), (4, 5), (4, 6)]
     slots = [parts.slot(rt, runs, heads, run, bh, tile) for rt in (0, 1) for run, bh in line]
     assert all(b - a >= tile for a, b in zip(slots, slots[1:]))
+
+
+def test_rows_that_the_token_arithmetic_cannot_tell_are_refused():
+    """row -> token is a 32-bit multiplication, exact for row * group < 2^32 up to the end of the last tile (128
+    rows), whatever kernel takes the call."""
+    from llmquant_b200 import native
+
+    lib = native.library()
+    for group, fits in ((65472, True), (65473, False), (65490, False), (65504, False)):
+        assert ((group + 128) * group < 2 ** 32) == fits  # (one token: as many rows as heads)
+        c = native.BlockKV(4096, 4096, 64, 64, 4096, 4096, 64, 8, 4, 1, 1, 128, 64, native.LQ_BF16)
+        assert (lib.lq_block_attn_scratch_bytes(ctypes.byref(c), group, 1) > 0) == fits
