@@ -114,9 +114,10 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 }
 
 // ---------------------------------------------------------------- how the line of units is cut
-// Per cent of a long line that the warps which run at once take. 70 / 80 / 90: one context of 131072 tokens
-// 62.3 / 62.6 / 63.9 us, 64 ragged sequences 62.6 / 63.7 / 67.5, 32 ragged sequences with their
-// append 56.9 / 56.8 / 59.3.
+// Per cent of a long line that the warps which run at once take: little enough that the short runs behind
+// them even out SMs of different speed. 70 / 80 / 90: one context of 131000 tokens 62.7 / 63.2 / 64.4 us, 64
+// ragged sequences 67.4 / 67.6 / 71.0, 32 ragged sequences with their append 54.6 / 54.6 / 57.0: 70 and 80
+// differ by less than 1 %, above that the last runs end late.
 constexpr int kFirst = 80;
 
 struct Shape {
@@ -267,9 +268,9 @@ __device__ __forceinline__ float largest_of(const uint32_t (&w)[N]) {
 
 // ---------------------------------------------------------------- main kernel
 // grid (runs of the line, row tiles), one warp. T is the type of q, out and the ring. Bound by the
-// latencies of a warp's units (12 warps on an SM, 1.8 instructions a cycle), by about 8 us before the
+// latencies of a warp's units (12 warps on an SM, 1.7 instructions a cycle), by about 8 us before the
 // first unit and in the join, and by SMs that stream at different speeds. One row each, 32 query heads
-// on 8, bf16, with the join: one context of 131000 tokens (268 MB) 64 us, 4.2 TB/s, 0.65 of a copy's
+// on 8, bf16, with the join: one context of 131000 tokens (268 MB) 63 us, 4.3 TB/s, 0.66 of a copy's
 // rate; 64 ragged contexts to 6000 with heads of 64 (299 MB) 68 us, 4.4 TB/s, 0.68. The same kernel
 // that only loads the codes takes 48 us instead of 53 for the long context, before the join.
 template <typename T, int D, int NT>

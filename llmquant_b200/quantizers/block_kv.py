@@ -402,10 +402,12 @@ class BlockKVCache(Cache):
             layer.crop(max_length)
 
 
-# Query tokens up to which `int_kv_attention` reads the codes; longer ones (prompts: chunks on top of
-# cached tokens come with a mask) read the cache back once and take transformers' SDPA. Measured from
-# an empty cache, 32 query heads of 128 on 8: 16 tokens 8.7 us by the codes and 10.7 read back, 32
-# tokens 13.7 and 11.0, 512 tokens 51 and 26.
+# Query tokens up to which `int_kv_attention` reads the codes; longer ones read the cache back once and take
+# transformers' SDPA. With several tokens that can only be a prompt on an empty cache (chunks on top of
+# cached tokens come with a mask, which the codes' kernels do not take). There a call takes 16 us by the
+# codes and 36 read back, the host's part of both, for 2 to 16 tokens of 1 and 8 sequences, 32 query
+# heads of 128 or 64 on 8, 16 on 2 and 8 on 8; the GPU itself needs 6 to 17 us by the codes and 4 to 6
+# read back, and from 128 tokens of 8 sequences (512 of one) on the codes lose the call as well: 54 against 37 us.
 ATTEND_TOKENS = 16
 
 
